@@ -9,6 +9,7 @@ Dense matrices are CUV's ``tensor<float, dev_memory_space, column_major>``: here
 logical shape ``(rows, cols)`` whose rows are contiguous (``stride(0) == 1``); make one with
 :func:`colmajor_empty` or :func:`to_device`.
 """
+import collections
 import ctypes
 
 import numpy as np
@@ -19,7 +20,8 @@ from ._capi import (CuvDiaError, MODE_EXACT, MODE_FAST, RF_ADD, RF_MEAN, RF_ADD_
 
 __all__ = ["dev_dia_matrix_f", "host_dia_matrix_f", "filter_factory", "convert", "pull", "save_dia_mat", "load_dia_mat", "dev_block_descriptor_f", "prod", "spmv", "densedense_to_dia", "reduce_to_col",
            "reduce_to_row", "avg_diagonals", "bias_sigmoid_sample", "bias_sigmoid_sample_sum", "prod_bias_sigmoid_sample", "axpby", "learn_step_weight_decay",
-           "learn_step_weight_decay_momentum", "colmajor_empty", "to_device", "to_host",
+           "learn_step_weight_decay_momentum", "embedding", "embedding_grad", "dropout", "dropout_grad", "token_logprob",
+           "token_logprob_grad", "TokenLogprob", "colmajor_empty", "to_device", "to_host",
            "launch_count", "plan_status", "raise_if_gave_up", "CuvDiaError", "MODE_EXACT", "MODE_FAST"]
 
 
@@ -43,9 +45,9 @@ def launch_count():
 
 # ---- dense column-major helpers ---------------------------------------------------------------------
 
-def colmajor_empty(rows, cols, device="cuda"):
+def colmajor_empty(rows, cols, device="cuda", dtype=None):
     torch = _torch()
-    return torch.empty((cols, rows), dtype=torch.float32, device=device).t()
+    return torch.empty((cols, rows), dtype=torch.float32 if dtype is None else dtype, device=device).t()
 
 
 def to_device(a, device="cuda"):
@@ -538,3 +540,182 @@ def learn_step_weight_decay_momentum(W, momentum, dW, learnrate, momentum_weight
     _capi.check(_capi.lib().cuvdia_learn_step_weight_decay_momentum_f32(
         _ptr(w), _ptr(m), _ptr(g), w.numel(), float(learnrate), float(momentum_weight), float(decay), _stream()))
     return W
+
+
+# ---- operators of a token model --------------------------------------------------------------------------------
+
+def _float_types():
+    torch = _torch()
+    return {torch.float32: _capi.T_F32, torch.float16: _capi.T_F16, torch.bfloat16: _capi.T_BF16}
+
+
+def _invalid(message):
+    raise CuvDiaError(_capi.ERR_INVALID, message)
+
+
+def _matrix(t, name, device=None, shape=None, dtype=None):
+    """Leading dimension of a column-major matrix in one of the float types; ``device``, ``shape``, ``dtype``: what it
+    has to share with the call's other operands."""
+    if not (isinstance(t, _torch().Tensor) and t.dim() == 2 and t.dtype in _float_types()):
+        _invalid(name + " must be a 2-D tensor of float32, float16 or bfloat16")
+    if dtype is not None and t.dtype != dtype:
+        _invalid("%s has type %s, not %s" % (name, t.dtype, dtype))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _invalid("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    rows, cols = t.shape
+    if rows > 1 and t.stride(0) != 1:
+        _invalid(name + " must be column-major (stride(0) == 1)")
+    ld = t.stride(1) if cols > 1 else max(rows, 1)
+    if rows < 1 or ld < rows:
+        _invalid(name + " has no rows or overlapping columns")
+    if max(ld, cols) > 2147483647:
+        _invalid(name + " has a dimension beyond 2^31 - 1")
+    _on_device(t, name, device)
+    return int(ld)
+
+
+def _vector(t, name, size, device):
+    """A packed float32 vector."""
+    if not (isinstance(t, _torch().Tensor) and t.dim() == 1 and t.dtype == _torch().float32 and t.is_contiguous()):
+        _invalid(name + " must be a contiguous 1-D float32 tensor")
+    if t.numel() != size:
+        _invalid("%s has %d elements, not %d" % (name, t.numel(), size))
+    _on_device(t, name, device)
+
+
+def _token_type(t, ncols, device):
+    torch = _torch()
+    if not (isinstance(t, torch.Tensor) and t.dim() == 1 and t.dtype in (torch.int32, torch.int64) and t.is_contiguous()):
+        _invalid("tokens must be a contiguous 1-D int32 or int64 tensor")
+    if t.numel() != ncols:
+        _invalid("tokens has %d elements, not one per column (%d)" % (t.numel(), ncols))
+    _on_device(t, "tokens", device)
+    return _capi.T_I32 if t.dtype == torch.int32 else _capi.T_I64
+
+
+def _on_device(t, name, device):
+    if not t.is_cuda:
+        _invalid(name + " must be a CUDA tensor")
+    if device is not None and t.device != device:
+        _invalid("%s is on %s, not on %s" % (name, t.device, device))
+
+
+def _call(device, name, *args):
+    """Calls an entry point with ``device`` current and on its current stream."""
+    torch = _torch()
+    if torch.cuda.current_device() == device.index:
+        _capi.check(getattr(_capi.lib(), name)(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            _capi.check(getattr(_capi.lib(), name)(*args, _stream()))
+
+
+def embedding(dst, table, tokens, scale=1.0):
+    """dst[:, j] = scale * table[:, tokens[j]]; a column of zeros where the token lies outside the table (padding).
+    ``table`` is units x vocab, ``dst`` units x ncols, column-major, both float32, float16 or bfloat16; ``tokens`` int32 or
+    int64, one per column."""
+    ldt = _matrix(table, "table")
+    dev, (units, vocab) = table.device, table.shape
+    if not isinstance(dst, _torch().Tensor) or dst.dim() != 2:
+        _invalid("dst must be a 2-D tensor")
+    ncols = dst.shape[1]
+    ldd = _matrix(dst, "dst", dev, (units, ncols), table.dtype)
+    tt = _token_type(tokens, ncols, dev)
+    if ncols == 0:
+        return dst
+    _call(dev, "cuvdia_embedding", _ptr(dst), ldd, _ptr(table), ldt, _float_types()[table.dtype], units, vocab, _ptr(tokens),
+          tt, ncols, float(scale))
+    return dst
+
+
+def embedding_grad(dtable, tokens, dout, factNew=1.0, factOld=0.0):
+    """dtable[:, v] = factOld*dtable[:, v] + factNew * sum of dout[:, j] over the positions j with tokens[j] == v: the
+    gradient of :func:`embedding` (``factNew`` = its scale) for the whole table, summed in 32 bits in ascending j.
+    ``factOld=0`` writes zeros into the columns of tokens that do not occur; ``factOld=1`` leaves those alone.  ``dtable`` has
+    the type of ``dout`` or float32."""
+    torch = _torch()
+    ldo = _matrix(dout, "dout")
+    dev, (units, ncols) = dout.device, dout.shape
+    if not isinstance(dtable, torch.Tensor) or dtable.dim() != 2 or dtable.dtype not in (dout.dtype, torch.float32):
+        _invalid("dtable must be a 2-D tensor of dout's type or float32")
+    vocab = dtable.shape[1]
+    ldt = _matrix(dtable, "dtable", dev, (units, vocab))
+    tt = _token_type(tokens, ncols, dev)
+    need = ctypes.c_longlong()
+    _capi.check(_capi.lib().cuvdia_embedding_grad_workspace(units, vocab, ncols, ctypes.byref(need)))
+    work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    types = _float_types()
+    _call(dev, "cuvdia_embedding_grad", _ptr(dtable), ldt, types[dtable.dtype], _ptr(dout), ldo, types[dout.dtype], units, vocab,
+          _ptr(tokens), tt, ncols, float(factNew), float(factOld), _ptr(work), need.value)
+    return dtable
+
+
+def dropout(dst, src, p, seed, step=0, col0=0, which=0, residual=None):
+    """dst = (u >= p ? src / (1 - p) : 0) [+ residual], u the uniform number :func:`fill_rnd_uniform` gives for the same
+    (seed, step, col0, which): no mask is stored, :func:`dropout_grad` draws the same one again.  float32, float16 or
+    bfloat16, all of one type; ``dst`` may be ``src`` or ``residual``."""
+    lds = _matrix(src, "src")
+    dev, (rows, ncols) = src.device, src.shape
+    ldd = _matrix(dst, "dst", dev, src.shape, src.dtype)
+    ldr = _matrix(residual, "residual", dev, src.shape, src.dtype) if residual is not None else 0
+    if ncols == 0:
+        return dst
+    d = _capi.Draw(int(seed), int(step), int(col0))
+    _call(dev, "cuvdia_dropout", _ptr(dst), ldd, _ptr(src), lds, _ptr(residual), ldr, _float_types()[src.dtype], rows, ncols,
+          float(p), ctypes.byref(d), int(which))
+    return dst
+
+
+def dropout_grad(dsrc, ddst, p, seed, step=0, col0=0, which=0):
+    """Gradient of :func:`dropout` with respect to ``src``, from the gradient ``ddst`` of its result and the same draw (the
+    gradient with respect to ``residual`` is ``ddst`` itself).  ``dsrc`` may be ``ddst``."""
+    return dropout(dsrc, ddst, p, seed, step, col0, which)
+
+
+TokenLogprob = collections.namedtuple("TokenLogprob", ["logp", "lse", "entropy", "top_logp", "top_index"])
+
+
+def token_logprob(logits, tokens=None, scale=1.0, entropy=False, top=0):
+    """Per column of ``logits`` (vocab x ncols, column-major; float32, float16 or bfloat16), under softmax(scale * logits):
+    ``logp`` of ``tokens[j]`` (0 where the token lies outside the vocabulary: padding), ``lse`` the log-sum-exp, ``entropy``,
+    and the ``top`` (at most 32) likeliest tokens in descending order, ties to the lowest token: ``top_logp``,
+    ``top_index`` of shape (top, ncols).  Returns a :class:`TokenLogprob` of new float32 (int32) tensors, None for what
+    was not asked for.  A logit of -inf is a forbidden token."""
+    torch = _torch()
+    ld = _matrix(logits, "logits")
+    dev, (vocab, ncols) = logits.device, logits.shape
+    tt = _token_type(tokens, ncols, dev) if tokens is not None else 0
+    top = int(top)
+    if not 0 <= top <= 32:
+        _invalid("0 <= top <= 32")
+    # one allocation for all results
+    n = ncols * (1 + (tokens is not None) + bool(entropy))
+    out = torch.empty(n + ncols * top, dtype=torch.float32, device=dev)
+    lse = out[:ncols]
+    logp = out[ncols:2 * ncols] if tokens is not None else None
+    ent = out[n - ncols:n] if entropy else None
+    top_logp = out[n:].view(ncols, top).t() if top else None
+    top_index = torch.empty((ncols, top), dtype=torch.int32, device=dev).t() if top else None
+    if ncols:
+        _call(dev, "cuvdia_token_logprob", _ptr(logits), ld, _float_types()[logits.dtype], vocab, ncols, _ptr(tokens), tt,
+              float(scale), _ptr(logp), _ptr(lse), _ptr(ent), top, _ptr(top_logp), _ptr(top_index))
+    return TokenLogprob(logp, lse, ent, top_logp, top_index)
+
+
+def token_logprob_grad(dlogits, logits, lse, tokens=None, dlogp=None, entropy=None, dentropy=None, scale=1.0):
+    """dlogits[v, j] = scale * (dlogp[j]*([v == tokens[j]] - p_v) - dentropy[j]*p_v*(log p_v + entropy[j])): the gradient of a
+    loss through :func:`token_logprob`'s ``logp`` (``tokens`` and ``dlogp``) and ``entropy`` (``entropy`` and ``dentropy``);
+    ``lse``, ``entropy`` are its results, ``scale`` its scale.  ``dlogits`` has the type of ``logits`` and may be ``logits``."""
+    ld = _matrix(logits, "logits")
+    dev, (vocab, ncols) = logits.device, logits.shape
+    ldd = _matrix(dlogits, "dlogits", dev, logits.shape, logits.dtype)
+    _vector(lse, "lse", ncols, dev)
+    tt = _token_type(tokens, ncols, dev) if tokens is not None else 0
+    for t, name in ((dlogp, "dlogp"), (entropy, "entropy"), (dentropy, "dentropy")):
+        if t is not None:
+            _vector(t, name, ncols, dev)
+    if ncols == 0:
+        return dlogits
+    _call(dev, "cuvdia_token_logprob_grad", _ptr(dlogits), ldd, _ptr(logits), ld, _float_types()[logits.dtype], vocab, ncols,
+          _ptr(tokens), tt, float(scale), _ptr(lse), _ptr(dlogp), _ptr(entropy), _ptr(dentropy))
+    return dlogits

@@ -10,7 +10,7 @@ LIB_PATH = os.path.join(_HERE, "libcuvdia.so")
 
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_NOMEM = range(5)
 MODE_EXACT, MODE_FAST = 0, 1
-T_F32, T_I32, T_U32, T_U8 = range(4)
+T_F32, T_I32, T_U32, T_U8, T_F16, T_BF16, T_I64 = range(7)
 (RF_ADD, RF_MEAN, RF_ADD_SQUARED, RF_MAX, RF_ARGMAX, RF_ARGMIN, RF_MIN, RF_MULT, RF_LOGADDEXP,
  RF_ADDEXP) = range(10)
 
@@ -55,6 +55,12 @@ SIGNATURES = {
     "cuvdia_binary_f32": (_i, [_vp, _vp, _vp, _i, _f, _f, _ll, _vp]),
     "cuvdia_fill_f32": (_i, [_vp, _f, _ll, _vp]),
     "cuvdia_sequence_f32": (_i, [_vp, _ll, _vp]),
+    "cuvdia_embedding": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _vp, _i, _i, _f, _vp]),
+    "cuvdia_embedding_grad_workspace": (_i, [_i, _i, _i, ctypes.POINTER(_ll)]),
+    "cuvdia_embedding_grad": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _i, _i, _f, _f, _vp, _ll, _vp]),
+    "cuvdia_dropout": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _f, _vp, _i, _vp]),
+    "cuvdia_token_logprob": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _f, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
+    "cuvdia_token_logprob_grad": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -438,4 +438,103 @@ int cuvdia_sequence_f32(float* dst, long long n, void* stream) {
     return launch_fill(dst, 0.f, 1, n, (cudaStream_t)stream);
 }
 
+static bool is_float_type(int t) { return t == CUVDIA_T_F32 || t == CUVDIA_T_F16 || t == CUVDIA_T_BF16; }
+static bool is_token_type(int t) { return t == CUVDIA_T_I32 || t == CUVDIA_T_I64; }
+static bool whole_elements(const void* p, int type) {
+    const uintptr_t size = type == CUVDIA_T_I64 ? 8 : type == CUVDIA_T_F16 || type == CUVDIA_T_BF16 ? 2 : 4;
+    return reinterpret_cast<uintptr_t>(p) % size == 0;
+}
+
+int cuvdia_embedding(void* dst, int ldd, const void* table, int ldt, int type, int units, int vocab, const void* tokens,
+                     int token_type, int ncols, float scale, void* stream) {
+    CUVDIA_REQUIRE(dst != nullptr && table != nullptr && tokens != nullptr);
+    CUVDIA_REQUIRE(is_float_type(type));
+    CUVDIA_REQUIRE(is_token_type(token_type));
+    CUVDIA_REQUIRE(whole_elements(dst, type) && whole_elements(table, type) && whole_elements(tokens, token_type));
+    CUVDIA_REQUIRE(units > 0 && vocab > 0 && ncols >= 0);
+    CUVDIA_REQUIRE(ldd >= units && ldt >= units);
+    if (ncols == 0) return CUVDIA_OK;
+    return launch_embedding(dst, ldd, table, ldt, type, units, vocab, tokens, token_type, ncols, scale, (cudaStream_t)stream);
+}
+
+int cuvdia_embedding_grad_workspace(int units, int vocab, int ncols, long long* bytes) {
+    CUVDIA_REQUIRE(bytes != nullptr);
+    CUVDIA_REQUIRE(units > 0 && vocab > 0 && ncols >= 0 && ncols <= (1 << 30));
+    *bytes = embedding_grad_bytes(units, vocab, ncols);
+    return CUVDIA_OK;
+}
+
+int cuvdia_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout, int ldo, int type, int units, int vocab,
+                          const void* tokens, int token_type, int ncols, float factNew, float factOld, void* workspace,
+                          long long workspace_bytes, void* stream) {
+    CUVDIA_REQUIRE(dtable != nullptr);
+    CUVDIA_REQUIRE(is_float_type(type));
+    CUVDIA_REQUIRE(grad_type == type || grad_type == CUVDIA_T_F32);
+    CUVDIA_REQUIRE(is_token_type(token_type));
+    CUVDIA_REQUIRE(units > 0 && vocab > 0 && ncols >= 0 && ncols <= (1 << 30));
+    CUVDIA_REQUIRE(ldt >= units);
+    CUVDIA_REQUIRE(whole_elements(dtable, grad_type));
+    if (ncols > 0) {
+        CUVDIA_REQUIRE(dout != nullptr && tokens != nullptr && workspace != nullptr);
+        CUVDIA_REQUIRE(ldo >= units);
+        CUVDIA_REQUIRE(whole_elements(dout, type) && whole_elements(tokens, token_type));
+        CUVDIA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
+        CUVDIA_REQUIRE(workspace_bytes >= embedding_grad_bytes(units, vocab, ncols));
+    }
+    return launch_embedding_grad(dtable, ldt, grad_type, dout, ldo, type, units, vocab, tokens, token_type, ncols, factNew,
+                                 factOld, workspace, (cudaStream_t)stream);
+}
+
+int cuvdia_dropout(void* dst, int ldd, const void* src, int lds, const void* residual, int ldr, int type, int rows,
+                   int ncols, float p, const cuvdia_draw* draw, int which, void* stream) {
+    CUVDIA_REQUIRE(dst != nullptr && src != nullptr && draw != nullptr);
+    CUVDIA_REQUIRE(is_float_type(type));
+    CUVDIA_REQUIRE(whole_elements(dst, type) && whole_elements(src, type) && whole_elements(residual, type));
+    CUVDIA_REQUIRE(rows > 0 && ncols >= 0);
+    CUVDIA_REQUIRE(ldd >= rows && lds >= rows && (residual == nullptr || ldr >= rows));
+    CUVDIA_REQUIRE(p >= 0.f && p <= 1.f);
+    CUVDIA_REQUIRE(which >= 0 && which < 65536);
+    CUVDIA_REQUIRE(draw->col0 >= 0 && draw->step < (1ull << 32));
+    if (ncols == 0) return CUVDIA_OK;
+    return launch_dropout(dst, ldd, src, lds, residual, ldr, type, rows, ncols, p, make_draw(draw, (unsigned)which),
+                          (cudaStream_t)stream);
+}
+
+int cuvdia_token_logprob(const void* logits, int ld, int type, int vocab, int ncols, const void* tokens, int token_type,
+                         float scale, float* logp, float* lse, float* entropy, int top, float* top_logp, int* top_index,
+                         void* stream) {
+    CUVDIA_REQUIRE(logits != nullptr);
+    CUVDIA_REQUIRE(is_float_type(type));
+    CUVDIA_REQUIRE(whole_elements(logits, type));
+    CUVDIA_REQUIRE(vocab > 0 && vocab <= (1 << 30) && ncols >= 0);
+    CUVDIA_REQUIRE(ld >= vocab);
+    CUVDIA_REQUIRE(scale > 0.f && scale <= 3.402823466e38f);
+    CUVDIA_REQUIRE((tokens == nullptr) == (logp == nullptr));
+    CUVDIA_REQUIRE(tokens == nullptr || (is_token_type(token_type) && whole_elements(tokens, token_type)));
+    CUVDIA_REQUIRE(top >= 0 && top <= 32);
+    CUVDIA_REQUIRE(top == 0 || (top_logp != nullptr && top_index != nullptr));
+    CUVDIA_REQUIRE(logp != nullptr || lse != nullptr || entropy != nullptr || top > 0);
+    if (ncols == 0) return CUVDIA_OK;
+    return launch_token_logprob(logits, ld, type, vocab, ncols, tokens, token_type, scale, logp, lse, entropy, top, top_logp,
+                                top_index, (cudaStream_t)stream);
+}
+
+int cuvdia_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld, int type, int vocab, int ncols,
+                              const void* tokens, int token_type, float scale, const float* lse, const float* dlogp,
+                              const float* entropy, const float* dentropy, void* stream) {
+    CUVDIA_REQUIRE(dlogits != nullptr && logits != nullptr && lse != nullptr);
+    CUVDIA_REQUIRE(is_float_type(type));
+    CUVDIA_REQUIRE(whole_elements(dlogits, type) && whole_elements(logits, type));
+    CUVDIA_REQUIRE(vocab > 0 && vocab <= (1 << 30) && ncols >= 0);
+    CUVDIA_REQUIRE(ld >= vocab && ldd >= vocab);
+    CUVDIA_REQUIRE(scale > 0.f && scale <= 3.402823466e38f);
+    CUVDIA_REQUIRE((tokens == nullptr) == (dlogp == nullptr));
+    CUVDIA_REQUIRE(tokens == nullptr || (is_token_type(token_type) && whole_elements(tokens, token_type)));
+    CUVDIA_REQUIRE((entropy == nullptr) == (dentropy == nullptr));
+    CUVDIA_REQUIRE(dlogp != nullptr || dentropy != nullptr);
+    if (ncols == 0) return CUVDIA_OK;
+    return launch_token_logprob_grad(dlogits, ldd, logits, ld, type, vocab, ncols, tokens, token_type, scale, lse, dlogp,
+                                     entropy, dentropy, (cudaStream_t)stream);
+}
+
 }  // extern "C"

@@ -187,5 +187,20 @@ int launch_axpby(float* dst, const float* x, const float* y, float a, float b, l
 int launch_learn_step(float* W, float* M, const float* dW, float a, float b, float c, long long n, cudaStream_t st);
 int launch_binary(float* dst, const float* x, const float* y, int op, float p, float p2, long long n, cudaStream_t st);
 int launch_fill(float* dst, float value, int sequence, long long n, cudaStream_t st);
+// token-model operators (types are CUVDIA_T_* codes the caller has checked)
+int launch_embedding(void* dst, int ldd, const void* table, int ldt, int type, int units, int vocab, const void* tokens,
+                     int token_type, int ncols, float scale, cudaStream_t st);
+long long embedding_grad_bytes(int units, int vocab, int ncols);
+int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout, int ldo, int type, int units, int vocab,
+                          const void* tokens, int token_type, int ncols, float fnew, float fold, void* workspace,
+                          cudaStream_t st);
+int launch_dropout(void* dst, int ldd, const void* src, int lds, const void* residual, int ldr, int type, int rows,
+                   int ncols, float p, const DrawParams& d, cudaStream_t st);
+int launch_token_logprob(const void* logits, int ld, int type, int vocab, int ncols, const void* tokens, int token_type,
+                         float scale, float* logp, float* lse, float* entropy, int top, float* top_logp, int* top_index,
+                         cudaStream_t st);
+int launch_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld, int type, int vocab, int ncols,
+                              const void* tokens, int token_type, float scale, const float* lse, const float* dlogp,
+                              const float* entropy, const float* dentropy, cudaStream_t st);
 int launch_selftest_wait(int* status, unsigned max_polls, cudaStream_t st);
 }  // namespace cuvdia

@@ -1,0 +1,120 @@
+// Element types of the token-model operators (fp32, fp16, bf16): conversion to and from the fp32 that everything is
+// computed in, and 16-byte vectors of them.  A store rounds once, to nearest even.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "cuvdia_internal.cuh"
+
+namespace cuvdia {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <class T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// two packed 16-bit elements <-> two floats
+template <class T> __device__ __forceinline__ float2 unpack2(unsigned w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned w) {
+    __half2 h;
+    *reinterpret_cast<unsigned*>(&h) = w;
+    return __half22float2(h);
+}
+template <class T> __device__ __forceinline__ unsigned pack2(float a, float b);
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// 16 bytes of T
+template <class T> struct Vec16 { static constexpr int N = 16 / (int)sizeof(T); };
+
+template <class T>
+__device__ __forceinline__ void unpack16(const uint4& r, float (&x)[Vec16<T>::N]) {
+    if constexpr (sizeof(T) == 4) {
+        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+    } else {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float2 f = unpack2<T>(w[q]);
+            x[2 * q] = f.x; x[2 * q + 1] = f.y;
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ uint4 pack16(const float (&x)[Vec16<T>::N]) {
+    if constexpr (sizeof(T) == 4) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    } else {
+        return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+    }
+}
+
+// N consecutive elements at p: one 128-bit access per 16 bytes (p 16-byte aligned), or, where ALIGNED is false or the
+// range ends inside, element by element up to `n` of them.
+template <class T, int N, bool ALIGNED>
+__device__ __forceinline__ void load_run(const T* __restrict__ p, int n, float (&x)[N]) {
+    constexpr int V = Vec16<T>::N;
+    static_assert(!ALIGNED || N % V == 0, "whole vectors");
+    if (ALIGNED && n >= N) {
+#pragma unroll
+        for (int q = 0; q < N / V; q++) {
+            float y[V];
+            unpack16<T>(*reinterpret_cast<const uint4*>(p + q * V), y);
+#pragma unroll
+            for (int e = 0; e < V; e++) x[q * V + e] = y[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = e < n ? to_f32(p[e]) : 0.f;
+    }
+}
+
+template <class T, int N, bool ALIGNED>
+__device__ __forceinline__ void store_run(T* __restrict__ p, int n, const float (&x)[N]) {
+    constexpr int V = Vec16<T>::N;
+    if (ALIGNED && n >= N) {
+#pragma unroll
+        for (int q = 0; q < N / V; q++) {
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) y[e] = x[q * V + e];
+            *reinterpret_cast<uint4*>(p + q * V) = pack16<T>(y);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) if (e < n) p[e] = from_f32<T>(x[e]);
+    }
+}
+
+// every column of a matrix starts on a 16-byte boundary
+inline bool columns16(const void* p, long long ld, int size) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+}
+
+inline int type_size(int type) {
+    return type == CUVDIA_T_F32 ? 4 : (type == CUVDIA_T_F16 || type == CUVDIA_T_BF16) ? 2 : 0;
+}
+
+// FN(T) for the element type `type` (checked by the caller)
+#define CUVDIA_FLOAT_TYPE(type, FN)                                          \
+    switch (type) {                                                          \
+        case CUVDIA_T_F32: { typedef float T; FN; break; }                   \
+        case CUVDIA_T_F16: { typedef __half T; FN; break; }                  \
+        default: { typedef __nv_bfloat16 T; FN; break; }                     \
+    }
+
+}  // namespace cuvdia

@@ -420,6 +420,71 @@ CUVDIA_API int cuvdia_binary_f32(float* dst, const float* x, const float* y, int
 CUVDIA_API int cuvdia_fill_f32(float* dst, float value, long long n, void* stream);
 CUVDIA_API int cuvdia_sequence_f32(float* dst, long long n, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a token model around the DIA layers: the input columns picked by token, dropout between
+ * the layers, and the softmax over a vocabulary at the end, each with its gradient.  No counterpart in
+ * CUV.  Matrices are column-major with a leading dimension, one batch column (token position) per
+ * column, as everywhere else; any leading dimension >= the row count and any alignment of whole
+ * elements is accepted (columns that start on 16-byte boundaries are the fast case), and rows beyond
+ * the row count are neither read nor written.  Element types: CUVDIA_T_F32, CUVDIA_T_F16,
+ * CUVDIA_T_BF16; everything is computed in 32 bits and rounded once.  Tokens: CUVDIA_T_I32 or
+ * CUVDIA_T_I64; a token outside [0, vocab) - padding - names no token, which is not an error.  Sums
+ * are taken in a fixed order (identical bits on every run).  No call allocates; all of them can be
+ * recorded into a graph.
+ * ------------------------------------------------------------------------------------------- */
+#define CUVDIA_T_F16  4
+#define CUVDIA_T_BF16 5
+#define CUVDIA_T_I64  6
+
+/* dst[:, j] = scale * table[:, tokens[j]], a column of zeros where the token is padding.  table is
+ * units x vocab, dst units x ncols; both of `type`.  dst must not overlap the table. */
+CUVDIA_API int cuvdia_embedding(void* dst, int ldd, const void* table, int ldt, int type, int units, int vocab,
+                                const void* tokens, int token_type, int ncols, float scale, void* stream);
+
+/* Gradient of the table: dtable[:, v] = factOld * dtable[:, v] + factNew * sum of dout[:, j] over the
+ * positions j with tokens[j] == v, in ascending j, for EVERY column v of the table.  factOld == 0:
+ * dtable is not read, columns of tokens that do not occur become zero.  factOld == 1: only columns of
+ * tokens that occur are touched (gradients accumulated over several batches).  grad_type is `type`
+ * (dout's) or CUVDIA_T_F32.  The positions are sorted by token inside the call; `workspace` is device
+ * memory of cuvdia_embedding_grad_workspace(units, vocab, ncols) bytes at least, 16-byte aligned, its
+ * contents undefined before and after; two calls that may overlap need two.  ncols <= 2^30. */
+CUVDIA_API int cuvdia_embedding_grad_workspace(int units, int vocab, int ncols, long long* bytes);
+CUVDIA_API int cuvdia_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout, int ldo, int type, int units,
+                                     int vocab, const void* tokens, int token_type, int ncols, float factNew,
+                                     float factOld, void* workspace, long long workspace_bytes, void* stream);
+
+/* dst = (u >= p ? src / (1 - p) : 0) + residual, u = the uniform number cuvdia_uniform_f32 gives for the
+ * element (draw, which): the mask is drawn in registers and never stored.  residual may be NULL (nothing
+ * is added).  The gradient with respect to src is the same call on the gradient of dst without residual;
+ * that of residual is the gradient of dst.  0 <= p <= 1; p = 1 drops everything.  A dropped element is zero
+ * whatever src holds (NaN and infinities too).  dst may be src or residual (the same pointer and leading
+ * dimension); it must not overlap them otherwise. */
+CUVDIA_API int cuvdia_dropout(void* dst, int ldd, const void* src, int lds, const void* residual, int ldr, int type,
+                              int rows, int ncols, float p, const cuvdia_draw* draw, int which, void* stream);
+
+/* Per column j of the logits (vocab x ncols, not written), with z = scale * logits[:, j]:
+ *   lse[j]      = log sum_v exp z_v
+ *   logp[j]     = z_{tokens[j]} - lse[j]; 0 where the token is padding
+ *   entropy[j]  = -sum_v p_v log p_v,  p_v = exp(z_v - lse[j])
+ *   top_index[k + top*j], top_logp[k + top*j], k = 0 .. top-1: the likeliest tokens in descending order, ties to the
+ *                 lowest token, and their log probabilities
+ * Any of lse, logp (with tokens) and entropy may be NULL, not all with top == 0; 0 <= top <= 32.  A logit of -inf is
+ * a forbidden token: probability zero, never among the likeliest; places left over hold index -1 and -inf.
+ * A column without any finite logit gives lse = logp = -inf, entropy 0.  A NaN or +inf logit makes lse, logp and
+ * entropy NaN (NaN is never among the likeliest).  scale is finite and positive. */
+CUVDIA_API int cuvdia_token_logprob(const void* logits, int ld, int type, int vocab, int ncols, const void* tokens,
+                                    int token_type, float scale, float* logp, float* lse, float* entropy, int top,
+                                    float* top_logp, int* top_index, void* stream);
+
+/* Gradient of a loss through logp and entropy of the call above:
+ *   dlogits[v, j] = scale * ( dlogp[j] * ([v == tokens[j]] - p_v) - dentropy[j] * p_v * (log p_v + entropy[j]) )
+ * lse and (with dentropy) entropy are that call's results.  dlogp (with tokens) or dentropy may be NULL, not
+ * both.  dlogp[j] is not used where the token is padding.  A column without any finite logit gets zeros.
+ * dlogits has the logits' type; it may be the logits themselves (the same pointer and leading dimension). */
+CUVDIA_API int cuvdia_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld, int type, int vocab, int ncols,
+                                         const void* tokens, int token_type, float scale, const float* lse,
+                                         const float* dlogp, const float* entropy, const float* dentropy, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
