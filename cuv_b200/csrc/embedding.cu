@@ -15,16 +15,16 @@ static inline int lanes_for(long long items) {
 // ---- lookup -----------------------------------------------------------------------------------------------------
 // `lanes` threads (a power of two) share a column, 256 / lanes columns a block; a thread moves up to four runs of N
 // elements of its column, all loads before the first store.
-template <class T, class I, int N, bool ALIGNED>
+template <class T, int N, bool ALIGNED>
 __global__ void __launch_bounds__(256)
 embedding_kernel(T* __restrict__ dst, long long ldd, const T* __restrict__ table, long long ldt, int units, int vocab,
-                 const I* __restrict__ tokens, int ncols, float scale, int lanes, int chunks) {
+                 const Tokens tokens, int ncols, float scale, int lanes, int chunks) {
     constexpr int U = 4;
     const unsigned group = blockIdx.x / (unsigned)chunks, chunk = blockIdx.x - group * (unsigned)chunks;
     const int sub = threadIdx.x / lanes, lane = threadIdx.x - sub * lanes;
     const long long col = (long long)group * (256 / lanes) + sub;
     if (col >= ncols) return;
-    const long long tok = (long long)tokens[col];
+    const long long tok = tokens[col];
     const bool there = tok >= 0 && tok < vocab;
     const T* from = table + (there ? tok : 0) * ldt;
     T* to = dst + col * ldd;
@@ -55,12 +55,9 @@ int launch_embedding(void* dst, int ldd, const void* table, int ldt, int type, i
     const long long chunks = (items + lanes - 1) / lanes, per = 256 / lanes;
     const long long blocks = (ncols + per - 1) / per * chunks;
     if (blocks > 2147483647LL) { set_last_error("embedding: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
-#define EMB_GO(I, N, A) embedding_kernel<T, I, N, A><<<(unsigned)blocks, 256, 0, st>>>((T*)dst, ldd, (const T*)table, ldt, \
-    units, vocab, (const I*)tokens, ncols, scale, lanes, (int)chunks)
-    CUVDIA_FLOAT_TYPE(type, {
-        if (token_type == CUVDIA_T_I32) { if (aligned) EMB_GO(int, Vec16<T>::N, true); else EMB_GO(int, 1, false); }
-        else { if (aligned) EMB_GO(long long, Vec16<T>::N, true); else EMB_GO(long long, 1, false); }
-    });
+#define EMB_GO(N, A) embedding_kernel<T, N, A><<<(unsigned)blocks, 256, 0, st>>>((T*)dst, ldd, (const T*)table, ldt, units, \
+    vocab, make_tokens(tokens, token_type), ncols, scale, lanes, (int)chunks)
+    CUVDIA_FLOAT_TYPE(type, { if (aligned) EMB_GO(Vec16<T>::N, true); else EMB_GO(1, false); });
 #undef EMB_GO
     count_launch();
     return check_launch("embedding_kernel");
@@ -73,22 +70,21 @@ int launch_embedding(void* dst, int ldd, const void* table, int ldt, int type, i
 // tokens stay in ascending position, so the sums below are taken in the same order on every run.
 constexpr int SORT_TILE = 4096, SORT_DIGITS = 512, SORT_THREADS = 256;
 
-template <class I>
-__device__ __forceinline__ int sort_key(const I* tokens, long long j, int vocab) {
-    const long long t = (long long)tokens[j];
+__device__ __forceinline__ int sort_key(const Tokens& tokens, long long j, int vocab) {
+    const long long t = tokens[j];
     return t >= 0 && t < vocab ? (int)t : vocab;
 }
 
 // the pair at place j of the pass's input: the tokens themselves in the first pass
-template <class I, bool FIRST>
-__device__ __forceinline__ void sort_pair(const I* tokens, const int* keys, const int* pos, int j, int vocab, int& key, int& at) {
+template <bool FIRST>
+__device__ __forceinline__ void sort_pair(const Tokens& tokens, const int* keys, const int* pos, int j, int vocab, int& key, int& at) {
     if (FIRST) { key = sort_key(tokens, j, vocab); at = j; }
     else       { key = keys[j]; at = pos[j]; }
 }
 
-template <class I, bool FIRST>
+template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_count_kernel(const I* __restrict__ tokens, const int* __restrict__ keys, int n, int vocab, int shift, int digits,
+sort_count_kernel(const Tokens tokens, const int* __restrict__ keys, int n, int vocab, int shift, int digits,
                   int tiles, int* __restrict__ counts) {
     __shared__ int hist[SORT_DIGITS];
     for (int d = threadIdx.x; d < digits; d += SORT_THREADS) hist[d] = 0;
@@ -126,9 +122,9 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ count
     for (long long k = first; k < last; k++) { const int v = counts[k]; counts[k] = run; run += v; }
 }
 
-template <class I, bool FIRST>
+template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS)
-sort_move_kernel(const I* __restrict__ tokens, const int* __restrict__ keys, const int* __restrict__ pos, int n, int vocab,
+sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* __restrict__ pos, int n, int vocab,
                  int shift, int digits, int tiles, const int* __restrict__ counts, int* __restrict__ keys_out,
                  int* __restrict__ pos_out) {
     constexpr int WARPS = SORT_THREADS / 32, PER = SORT_TILE / SORT_THREADS;
@@ -143,7 +139,7 @@ sort_move_kernel(const I* __restrict__ tokens, const int* __restrict__ keys, con
     for (int r = 0; r < PER; r++) {
         const int j = first + r * 32;
         key[r] = at[r] = 0;
-        if (j < n) sort_pair<I, FIRST>(tokens, keys, pos, j, vocab, key[r], at[r]);
+        if (j < n) sort_pair<FIRST>(tokens, keys, pos, j, vocab, key[r], at[r]);
     }
 #pragma unroll
     for (int r = 0; r < PER; r++) {
@@ -311,19 +307,17 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     int* pos[2] = {(int*)(ws + g.pos[0]), (int*)(ws + g.pos[1])};
     int* counts = (int*)(ws + g.counts);
     float* partial = (float*)(ws + g.partial);
+    const Tokens toks = make_tokens(tokens, token_type);
     int src = 0;
     for (int p = 0; p < g.passes && ncols > 0; p++) {
         const int shift = p * g.digit_bits, digits = 1 << g.digit_bits;
-#define SORT_GO(I, F) do {                                                                                                  \
-        sort_count_kernel<I, F><<<g.tiles, SORT_THREADS, 0, st>>>((const I*)tokens, keys[src], ncols, vocab, shift, digits, \
-                                                                  g.tiles, counts);                                         \
-        sort_scan_kernel<<<1, 1024, 0, st>>>(counts, (long long)digits * g.tiles);                                          \
-        sort_move_kernel<I, F><<<g.tiles, SORT_THREADS, 0, st>>>((const I*)tokens, keys[src], pos[src], ncols, vocab, shift, \
-                                                                 digits, g.tiles, counts, keys[1 - src], pos[1 - src]);     \
+#define SORT_GO(F) do {                                                                                                  \
+        sort_count_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], ncols, vocab, shift, digits, g.tiles, counts); \
+        sort_scan_kernel<<<1, 1024, 0, st>>>(counts, (long long)digits * g.tiles);                                       \
+        sort_move_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], pos[src], ncols, vocab, shift, digits,    \
+                                                              g.tiles, counts, keys[1 - src], pos[1 - src]);             \
     } while (0)
-        if (p > 0) SORT_GO(int, false);
-        else if (token_type == CUVDIA_T_I32) SORT_GO(int, true);
-        else SORT_GO(long long, true);
+        if (p == 0) SORT_GO(true); else SORT_GO(false);
 #undef SORT_GO
         count_launch(3);
         int rc = check_launch("sort kernels of embedding_grad");

@@ -109,12 +109,22 @@ inline int type_size(int type) {
     return type == CUVDIA_T_F32 ? 4 : (type == CUVDIA_T_F16 || type == CUVDIA_T_BF16) ? 2 : 0;
 }
 
-// FN(T) for the element type `type` (checked by the caller)
-#define CUVDIA_FLOAT_TYPE(type, FN)                                          \
-    switch (type) {                                                          \
-        case CUVDIA_T_F32: { typedef float T; FN; break; }                   \
-        case CUVDIA_T_F16: { typedef __half T; FN; break; }                  \
-        default: { typedef __nv_bfloat16 T; FN; break; }                     \
+// token j of a vector of 32- or 64-bit integers
+struct Tokens {
+    const void* p;
+    bool wide;
+    __device__ __forceinline__ long long operator[](long long j) const {
+        return wide ? static_cast<const long long*>(p)[j] : static_cast<const int*>(p)[j];
+    }
+};
+inline Tokens make_tokens(const void* p, int token_type) { return {p, token_type == CUVDIA_T_I64}; }
+
+// the statements, with T the element type `type` (checked by the caller)
+#define CUVDIA_FLOAT_TYPE(type, ...) \
+    switch (type) { \
+        case CUVDIA_T_F32: { typedef float T; __VA_ARGS__; break; } \
+        case CUVDIA_T_F16: { typedef __half T; __VA_ARGS__; break; } \
+        default: { typedef __nv_bfloat16 T; __VA_ARGS__; break; } \
     }
 
 }  // namespace cuvdia
