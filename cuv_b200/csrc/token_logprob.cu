@@ -45,6 +45,25 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
     return a;
 }
 
+// the largest of a vector's elements, NaN left out
+__device__ __forceinline__ float max_raw(const uint4& r, float) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+}
+#define CUVDIA_RAW16(H, H2)                                                                                                    \
+    __device__ __forceinline__ float max_raw(const uint4& r, H) {                                                              \
+        const H2* h = reinterpret_cast<const H2*>(&r);                                                                         \
+        const H2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));                                                        \
+        return fmaxf(to_f32(m.x), to_f32(m.y));                                                                                \
+    }
+CUVDIA_RAW16(__half, __half2)
+CUVDIA_RAW16(__nv_bfloat16, __nv_bfloat162)
+#undef CUVDIA_RAW16
+
+template <class T> __device__ __forceinline__ unsigned minus_inf_word();
+template <> __device__ __forceinline__ unsigned minus_inf_word<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ unsigned minus_inf_word<__half>() { return 0xfc00fc00u; }
+template <> __device__ __forceinline__ unsigned minus_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
+
 // ---- the likeliest tokens ------------------------------------------------------------------------------------------
 // A candidate is one 64-bit number that orders like (logit descending, index ascending): the larger, the better; 0 = none.
 // NaN and -inf are never candidates.
@@ -60,14 +79,15 @@ __device__ __forceinline__ float key_value(Key k) {             // -inf for "non
 }
 __device__ __forceinline__ int key_index(Key k) { return k == 0 ? -1 : (int)~(unsigned)k; }
 
-// 32 candidates, one a lane, put in descending order (bitonic network)
-__device__ __forceinline__ Key sort_desc(Key k) {
+// 32 numbers, one a lane, put in descending order (bitonic network); K is Key, or the upper word of one
+template <class K>
+__device__ __forceinline__ K sort_desc(K k) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int n = 2; n <= 32; n *= 2)
 #pragma unroll
         for (int s = n / 2; s > 0; s /= 2) {
-            const Key o = __shfl_xor_sync(0xffffffffu, k, s);
+            const K o = __shfl_xor_sync(0xffffffffu, k, s);
             const bool upper = (lane & s) != 0, descending = (lane & n) == 0 || n == 32;
             k = (o > k) == (upper != descending) ? o : k;
         }
@@ -75,30 +95,46 @@ __device__ __forceinline__ Key sort_desc(Key k) {
 }
 
 // the best 32 of two descending lists, in descending order
-__device__ __forceinline__ Key merge_desc(Key a, Key b) {
+template <class K>
+__device__ __forceinline__ K merge_desc(K a, K b) {
     const int lane = threadIdx.x & 31;
-    const Key r = __shfl_sync(0xffffffffu, b, 31 - lane);
+    const K r = __shfl_sync(0xffffffffu, b, 31 - lane);
     a = r > a ? r : a;
 #pragma unroll
     for (int s = 16; s > 0; s /= 2) {
-        const Key o = __shfl_xor_sync(0xffffffffu, a, s);
+        const K o = __shfl_xor_sync(0xffffffffu, a, s);
         a = (o > a) == ((lane & s) == 0) ? o : a;
     }
     return a;
 }
 
-// A warp's best candidates so far: a descending list (one a lane), and up to 63 more in shared memory that wait to be sorted
-// in, 32 at a time.  `bar` is the k-th best of the list: what a new one has to beat.  `floor` is a lower bound on the
-// column's k-th best logit that the warps of the block raise together.
+// the best 32 of the descending lists of n warps, pairwise through shared memory: the result is warp 0's
+template <class K>
+__device__ __forceinline__ K merge_warps(K mine, K (*lists)[32], int n) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    lists[warp][lane] = mine;
+    __syncthreads();
+    for (int half = n / 2; half > 0; half /= 2) {
+        if (warp < half) lists[warp][lane] = mine = merge_desc(mine, lists[warp + half][lane]);
+        __syncthreads();
+    }
+    return mine;
+}
+
+// The best 32 of a descending list and 32 candidates in any order.  Called, not inlined: it is rare and long, and copies of it
+// cost more in instruction fetches than the calls.
+__device__ __noinline__ Key absorb32(Key list, Key batch) { return merge_desc(list, sort_desc(batch)); }
+__device__ __noinline__ unsigned sort_maxima(unsigned k) { return sort_desc(k); }
+
+// A warp's best candidates: a descending list (one a lane), and up to 63 more in shared memory that wait to be sorted in,
+// 32 at a time.  `bar` is the k-th best of the list: what a new one has to beat.
 struct Top {
     Key list, bar;
-    float bar_v;
     int waiting;
-    __device__ __forceinline__ void clear() { list = bar = 0; bar_v = -INFINITY; waiting = 0; }
+    __device__ __forceinline__ void clear() { list = bar = 0; waiting = 0; }
     __device__ __forceinline__ void absorb(Key batch, int k) {
-        list = merge_desc(list, sort_desc(batch));
+        list = absorb32(list, batch);
         bar = __shfl_sync(0xffffffffu, list, k - 1);
-        bar_v = key_value(bar);
     }
     // at most one candidate per lane (0: none)
     __device__ __forceinline__ void push(Key key, Key* buffer, int k) {
@@ -123,43 +159,69 @@ struct Top {
     }
 };
 
-// ---- one pass over a column -------------------------------------------------------------------------------------------
-__device__ __forceinline__ float max_raw(const uint4& r, float) {
-    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
-}
-__device__ __forceinline__ float min_raw(const uint4& r, float) {
-    return fminf(fminf(__uint_as_float(r.x), __uint_as_float(r.y)), fminf(__uint_as_float(r.z), __uint_as_float(r.w)));
-}
-#define CUVDIA_RAW16(H, H2)                                                                                                    \
-    __device__ __forceinline__ float max_raw(const uint4& r, H) {                                                              \
-        const H2* h = reinterpret_cast<const H2*>(&r);                                                                         \
-        const H2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));                                                        \
-        return fmaxf(to_f32(m.x), to_f32(m.y));                                                                                \
-    }                                                                                                                          \
-    __device__ __forceinline__ float min_raw(const uint4& r, H) {                                                              \
-        const H2* h = reinterpret_cast<const H2*>(&r);                                                                         \
-        const H2 m = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));                                                        \
-        return fminf(to_f32(m.x), to_f32(m.y));                                                                                \
+// The candidates among a thread's own vectors, looked at a second time once `least` is known, a lower bound on the k-th best
+// logit of all: only the few threads whose largest logit reaches it have any, and what they read again lies in L2.
+// xv: the column's whole vectors, the thread's own being first, first + step, .. below last.
+template <class T>
+__device__ __forceinline__ void collect(Top& top, int k, Key* buffer, float least, float largest, const uint4* xv, int first,
+                                        int last, int step, int head) {
+    constexpr int V = Vec16<T>::N, U = 4;
+    const bool any = largest >= least && largest > -INFINITY;
+    const unsigned nothing = minus_inf_word<T>();
+    if (!__any_sync(0xffffffffu, any)) return;
+    const int lane = threadIdx.x & 31, rounds = (last - (first - lane) + step - 1) / step;      // the same in all lanes
+    for (int r = 0; r < rounds; r += U) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int v = first + (r + u) * step;
+            raw[u] = any && r + u < rounds && v < last ? xv[v] : make_uint4(nothing, nothing, nothing, nothing);
+        }
+        unsigned hits = 0;                                      // bit u * V + e: element e of vector u reaches the bound
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float m = max_raw(raw[u], T());
+            if (m >= least && m > -INFINITY) {
+                float x[V];
+                unpack16<T>(raw[u], x);
+#pragma unroll
+                for (int e = 0; e < V; e++) hits |= x[e] >= least && x[e] > -INFINITY ? 1u << (u * V + e) : 0u;
+            }
+        }
+        while (__any_sync(0xffffffffu, hits != 0)) {
+            Key key = 0;
+            if (hits) {
+                const int slot = __ffs(hits) - 1;
+                hits &= hits - 1;
+                const int at = (first + (r + slot / V) * step) * V + slot % V;
+                key = make_key(to_f32(reinterpret_cast<const T*>(xv)[at]), at + head);     // the registers cannot be indexed
+            }
+            top.push(key, buffer, k);
+        }
     }
-CUVDIA_RAW16(__half, __half2)
-CUVDIA_RAW16(__nv_bfloat16, __nv_bfloat162)
-#undef CUVDIA_RAW16
+}
 
-template <class T> __device__ __forceinline__ unsigned minus_inf_word();
-template <> __device__ __forceinline__ unsigned minus_inf_word<float>() { return 0xff800000u; }
-template <> __device__ __forceinline__ unsigned minus_inf_word<__half>() { return 0xfc00fc00u; }
-template <> __device__ __forceinline__ unsigned minus_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
-
+// ---- one pass over a column -------------------------------------------------------------------------------------------
 // The sums of a thread as pairs, so that two elements share an instruction.
 struct Sums { float m; float2 s, t; };
 
+// The 32 threads' sums as one, in all lanes: relative to the warp's maximum first, so that only one rescaling each is needed.
 template <bool ENT>
-__device__ __forceinline__ Stat fold(const Sums& a) {
-    return {a.m, a.s.x + a.s.y, ENT ? a.t.x + a.t.y : 0.f};
+__device__ __forceinline__ Stat join_warp(Sums& a, float c) {
+    float m;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(a.m));
+    Stat r = {a.m, a.s.x + a.s.y, ENT ? a.t.x + a.t.y : 0.f};
+    rescale(r, m, c);
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, s);
+        if (ENT) r.t += __shfl_xor_sync(0xffffffffu, r.t, s);
+    }
+    return r;
 }
 
-// Adds U vectors to a thread's sums.  The exponents of an ordinary chunk are not cut (see LEAST): a chunk is cut only if its
-// smallest logit is so far below the maximum that an exponent times its power could be 0 * -inf.
+// Adds U vectors to a thread's sums, two elements an instruction.  An exponent of -inf (a forbidden token) times its power of
+// zero is NaN; such a chunk is summed once more with its exponents cut (see LEAST), the others need no test per element.
 template <class T, bool ENT, int U>
 __device__ __forceinline__ void add_chunk(Sums& a, float m, const uint4 (&raw)[U], float c) {
     constexpr int V = Vec16<T>::N;
@@ -173,70 +235,32 @@ __device__ __forceinline__ void add_chunk(Sums& a, float m, const uint4 (&raw)[U
     }
     const float m0 = shift(a.m);
     const float2 minus = make_float2(-m0, -m0), by = make_float2(c, c);
-    bool cut = false;
-    if (ENT) {
-        float low = min_raw(raw[0], T());
+    float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int u = 1; u < U; u++) low = fminf(low, min_raw(raw[u], T()));
-        cut = (low - m0) * c < LEAST;
+    for (int u = 0; u < U; u++) {
+        float x[V];
+        unpack16<T>(raw[u], x);
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), minus), by);
+            const float2 p = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+            a.s = __fadd2_rn(a.s, p);
+            if (ENT) t = __ffma2_rn(p, d, t);
+        }
     }
-    auto sum = [&](auto with_cut) {
+    if (ENT) {
+        if (t.x + t.y != t.x + t.y) {
+            t = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            float x[V];
-            unpack16<T>(raw[u], x);
+            for (int u = 0; u < U; u++) {
+                float x[V];
+                unpack16<T>(raw[u], x);
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), minus), by);
-                const float2 p = make_float2(exp2_approx(d.x), exp2_approx(d.y));
-                a.s = __fadd2_rn(a.s, p);
-                if (ENT) {
-                    if (decltype(with_cut)::value) d = make_float2(fmaxf(d.x, LEAST), fmaxf(d.y, LEAST));
-                    a.t = __ffma2_rn(p, d, a.t);
-                }
+                for (int e = 0; e < V; e++) { const float d = (x[e] - m0) * c; t.x = fmaf(exp2_approx(d), fmaxf(d, LEAST), t.x); }
             }
         }
-    };
-    if (ENT && cut) sum(std::true_type()); else sum(std::false_type());
-}
-
-// Offers a chunk's elements to the warp's list.  x0: the column; first: the thread's first whole vector, later ones `step`
-// vectors apart; v1: the first vector behind the part.
-template <class T, int U>
-__device__ __forceinline__ void offer_chunk(Top& top, int k, Key* buffer, unsigned* floor, float m, const uint4 (&raw)[U],
-                                            const T* x0, long long first, int step, int head) {
-    constexpr int V = Vec16<T>::N;
-    if (top.bar == 0 && top.waiting == 0) {
-        // Nothing met yet: the k-th largest of the 32 lanes' maxima bounds the k-th best from below.
-        const Key sorted = sort_desc(m > -INFINITY ? make_key(m, 0) : 0);
-        const float kth = key_value(__shfl_sync(0xffffffffu, sorted, k - 1));
-        if ((threadIdx.x & 31) == 0 && kth > -INFINITY) atomicMax(floor, (unsigned)(make_key(kth, 0) >> 32));
-        __syncwarp();
+        a.t.x += t.x; a.t.y += t.y;
     }
-    const unsigned fl = *(volatile unsigned*)floor;
-    const float least = fmaxf(top.bar_v, fl ? key_value((Key)fl << 32) : -INFINITY);
-    unsigned hits = 0;
-    if (m >= least) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            float x[V];
-            unpack16<T>(raw[u], x);
-#pragma unroll
-            for (int e = 0; e < V; e++) hits |= (x[e] >= least && x[e] > -INFINITY) ? 1u << (u * V + e) : 0u;
-        }
-    }
-    const Key before = top.bar;
-    while (__any_sync(0xffffffffu, hits != 0)) {
-        Key key = 0;
-        if (hits) {
-            const int slot = __ffs(hits) - 1;
-            hits &= hits - 1;
-            const int at = (int)((first + (long long)(slot / V) * step) * V) + head + slot % V;
-            key = make_key(to_f32(x0[at]), at);                 // a second look: the registers cannot be indexed
-        }
-        top.push(key, buffer, k);
-    }
-    if (top.bar != before && (threadIdx.x & 31) == 0) atomicMax(floor, (unsigned)(top.bar >> 32));
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -290,25 +314,20 @@ __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col
 // alone are too few to fill the GPU: its blocks leave their sums and lists in the first block's shared memory, which joins
 // them, so that there is one launch and no scratch memory.
 template <class T, bool ENT, bool TOP, int TEAM>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 token_logprob_kernel(const LogprobArgs q, int parts) {
     constexpr int V = Vec16<T>::N, U = 4, WARPS = 8, STEP = TEAM;
     __shared__ Stat stats[WARPS], part_stats[WARPS];
     __shared__ Key lists[TOP ? WARPS : 1][32], part_lists[TOP ? WARPS : 1][32], buffers[TOP ? WARPS : 1][64];
-    __shared__ unsigned floors[TOP ? WARPS : 1];
+    __shared__ unsigned maxima[TOP ? WARPS : 1][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = TEAM == 256 ? blockIdx.x % (unsigned)parts : 0;
     const long long col = TEAM == 256 ? blockIdx.x / (unsigned)parts : (long long)blockIdx.x * WARPS + warp;
     if (TEAM == 256 && parts > 1) cluster_arrive();             // waited for before the first remote store: all blocks run then
-    if (TOP) {
-        if (threadIdx.x < WARPS) floors[threadIdx.x] = 0;
-        __syncthreads();
-    }
     if (col >= q.ncols) return;
     const T* x0 = (const T*)q.logits + col * q.ld;
     const float c = q.scale * LOG2E;
     const int tid = TEAM == 256 ? threadIdx.x : lane;
-    unsigned* floor = &floors[TOP ? (TEAM == 256 ? 0 : warp) : 0];
     Key* buffer = buffers[TOP ? warp : 0];
     // whole 16-byte vectors of the column, behind `head` elements and before the rest
     const int head = min(q.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)));
@@ -316,16 +335,19 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     const uint4* xv = reinterpret_cast<const uint4*>(x0 + head);
     const int v0 = (int)((long long)nvec * part / parts), v1 = (int)((long long)nvec * (part + 1) / parts);
     Sums a = {-INFINITY, {0.f, 0.f}, {0.f, 0.f}};
-    Top best;
-    best.clear();
     const unsigned nothing = minus_inf_word<T>();
     uint4 next[U];
+    const uint4* from = xv + v0 + tid;                          // the chunk being fetched
     auto fetch = [&](int i) {
+        if (i + STEP * U <= v1) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int v = i + u * STEP + tid;
-            next[u] = v < v1 ? __ldg(xv + v) : make_uint4(nothing, nothing, nothing, nothing);
+            for (int u = 0; u < U; u++) next[u] = __ldg(from + u * STEP);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                next[u] = i + u * STEP + tid < v1 ? __ldg(from + u * STEP) : make_uint4(nothing, nothing, nothing, nothing);
         }
+        from += STEP * U;
     };
     fetch(v0);
     for (int i = v0; i < v1; i += STEP * U) {
@@ -337,51 +359,53 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
 #pragma unroll
         for (int u = 1; u < U; u++) m = fmaxf(m, max_raw(raw[u], T()));
         add_chunk<T, ENT, U>(a, m, raw, c);
-        // later elements have higher indices, so a tie with the bar is not a candidate
-        if (TOP && __any_sync(0xffffffffu, m > best.bar_v)) offer_chunk<T, U>(best, q.top, buffer, floor, m, raw, x0, i + tid, STEP, head);
     }
+    float edge = -INFINITY;                                     // of the ends: one element a lane at most
+    int edge_at = -1;
     if (part == 0 && (TEAM == 32 || warp == 0) && head + rest > 0) {       // the ends, element by element
-        const int at = lane < head ? lane : lane >= 16 && lane - 16 < rest ? head + nvec * V + lane - 16 : -1;
-        const float x = at >= 0 ? to_f32(x0[at]) : -INFINITY;
-        Stat b = {fmaxf(x, -INFINITY), 0.f, 0.f};               // NaN: leaves the maximum to the others
-        const float d = (x - shift(b.m)) * c;
+        edge_at = lane < head ? lane : lane >= 16 && lane - 16 < rest ? head + nvec * V + lane - 16 : -1;
+        edge = edge_at >= 0 ? to_f32(x0[edge_at]) : -INFINITY;
+        Stat b = {fmaxf(edge, -INFINITY), 0.f, 0.f};            // NaN: leaves the maximum to the others
+        const float d = (edge - shift(b.m)) * c;
         b.s = exp2_approx(d);
         b.t = b.s * fmaxf(d, LEAST);
-        const Stat joined = merge(fold<ENT>(a), b, c);
+        const Stat joined = merge({a.m, a.s.x + a.s.y, a.t.x + a.t.y}, b, c);
         a = {joined.m, {joined.s, 0.f}, {joined.t, 0.f}};
-        if (TOP) best.push(x > -INFINITY ? make_key(x, at) : 0, buffer, q.top);
     }
-    if (TOP) best.finish(buffer, q.top);
-    Stat st = fold<ENT>(a);
-#pragma unroll
-    for (int s = 16; s > 0; s /= 2) {
-        Stat b;
-        b.m = __shfl_xor_sync(0xffffffffu, st.m, s); b.s = __shfl_xor_sync(0xffffffffu, st.s, s);
-        b.t = ENT ? __shfl_xor_sync(0xffffffffu, st.t, s) : 0.f;
-        st = merge(st, b, c);
+    Key list = 0;
+    if (TOP) {
+        // The k-th largest of the threads' largest logits bounds the k-th best from below, and few logits reach it.
+        const unsigned own = a.m > -INFINITY ? (unsigned)(make_key(a.m, 0) >> 32) : 0;
+        unsigned sorted = sort_maxima(own);
+        if (TEAM == 256) {
+            sorted = merge_warps(sorted, maxima, WARPS);
+            if (warp == 0) maxima[0][lane] = sorted;
+            __syncthreads();
+            sorted = maxima[0][lane];
+        }
+        const float least = key_value((Key)__shfl_sync(0xffffffffu, sorted, q.top - 1) << 32);
+        Top best;
+        best.clear();
+        collect<T>(best, q.top, buffer, least, a.m, xv, v0 + tid, v1, STEP, head);
+        const bool hit = edge >= least && edge > -INFINITY;
+        if (__any_sync(0xffffffffu, hit)) best.push(hit ? make_key(edge, edge_at) : 0, buffer, q.top);
+        best.finish(buffer, q.top);
+        list = best.list;
     }
-    if (TEAM == 32) { write_column<T, ENT, TOP>(q, col, x0, st, best.list); return; }
+    Stat st = join_warp<ENT>(a, c);
+    if (TEAM == 32) { write_column<T, ENT, TOP>(q, col, x0, st, list); return; }
 
-    // the block's warps, pairwise
-    auto join = [&](Stat* ss, Key (*ls)[32], int n) {
-        if (lane == 0) ss[warp] = st;
-        if (TOP) ls[warp][lane] = best.list;
+    // the sums of n warps, in warp 0
+    auto join = [&](int n) {
+        if (lane == 0) stats[warp] = st;
         __syncthreads();
-        if (TOP) {
-            for (int half = n / 2; half > 0; half /= 2) {
-                if (warp < half) {
-                    best.list = merge_desc(best.list, ls[warp + half][lane]);
-                    ls[warp][lane] = best.list;
-                }
-                __syncthreads();
-            }
-        }
         if (warp == 0) {
-            st = ss[0];
-            for (int w = 1; w < n; w++) st = merge(st, ss[w], c);
+            st = stats[0];
+            for (int w = 1; w < n; w++) st = merge(st, stats[w], c);
         }
+        if (TOP) list = merge_warps(list, lists, n);
     };
-    join(stats, lists, WARPS);
+    join(WARPS);
     if (parts > 1) {
         cluster_wait();
         if (warp == 0) {
@@ -389,18 +413,17 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
                 const unsigned to = in_first_block(&part_stats[part]);
                 store_remote(to, __float_as_uint(st.m)); store_remote(to + 4, __float_as_uint(st.s)); store_remote(to + 8, __float_as_uint(st.t));
             }
-            if (TOP) store_remote(in_first_block(&part_lists[part][lane]), best.list);
+            if (TOP) store_remote(in_first_block(&part_lists[part][lane]), list);
         }
         cluster_arrive();
         cluster_wait();
         if (part != 0) return;
-        const Stat mine = part_stats[min(warp, parts - 1)];
-        st = mine;
-        if (TOP) best.list = part_lists[min(warp, parts - 1)][lane];
+        st = part_stats[min(warp, parts - 1)];
+        if (TOP) list = part_lists[min(warp, parts - 1)][lane];
         __syncthreads();
-        join(stats, lists, parts);
+        join(parts);
     }
-    if (warp == 0) write_column<T, ENT, TOP>(q, col, x0, st, best.list);
+    if (warp == 0) write_column<T, ENT, TOP>(q, col, x0, st, list);
 }
 
 template <class T, bool ENT, bool TOP>
@@ -414,8 +437,15 @@ static int logprob_go(const LogprobArgs& q, cudaStream_t st) {
         CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, TOP, 32>, q, 1));
         return CUVDIA_OK;
     }
+    // Waves of blocks (four fit an SM) times what a block takes: its chunks of 1024 vectors and about one chunk's time to
+    // start and to join its warps, two with a list of candidates.
     int parts = 1;
-    while (parts < 8 && (long long)q.ncols * parts < 16 * sm_count() && nvec / (2 * parts) >= 1024) parts *= 2;
+    long long best = 0;
+    for (int p = 1; p <= 8; p *= 2) {
+        const long long slots = 4 * sm_count(), waves = ((long long)q.ncols * p + slots - 1) / slots;
+        const long long cost = waves * ((nvec + 1024 * p - 1) / (1024 * p) + (TOP ? 2 : 1));
+        if (p == 1 || cost < best) { parts = p; best = cost; }
+    }
     if ((long long)q.ncols * parts > 2147483647LL) { set_last_error("token_logprob: too many columns"); return CUVDIA_ERR_UNSUPPORTED; }
     cfg.gridDim = dim3((unsigned)(q.ncols * parts));
     cudaLaunchAttribute cluster;
