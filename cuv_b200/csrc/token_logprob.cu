@@ -159,44 +159,48 @@ struct Top {
     }
 };
 
-// The candidates among a thread's own vectors, looked at a second time once `least` is known, a lower bound on the k-th best
-// logit of all: only the few threads whose largest logit reaches it have any, and what they read again lies in L2.
-// xv: the column's whole vectors, the thread's own being first, first + step, .. below last.
+// The candidates among a warp's vectors, looked at a second time once `least` is known, a lower bound on the k-th best logit of
+// all: only the few threads whose largest logit reaches it own any, and what is read again lies in L2.  The warp goes through
+// the vectors of one such thread after the other, 64 at a time.  xv: the column's whole vectors; the warp's own are
+// start + lane, start + lane + step, .. below last.
 template <class T>
-__device__ __forceinline__ void collect(Top& top, int k, Key* buffer, float least, float largest, const uint4* xv, int first,
+__device__ __forceinline__ void collect(Top& top, int k, Key* buffer, float least, float largest, const uint4* xv, int start,
                                         int last, int step, int head) {
-    constexpr int V = Vec16<T>::N, U = 4;
-    const bool any = largest >= least && largest > -INFINITY;
+    constexpr int V = Vec16<T>::N, U = 2;
     const unsigned nothing = minus_inf_word<T>();
-    if (!__any_sync(0xffffffffu, any)) return;
-    const int lane = threadIdx.x & 31, rounds = (last - (first - lane) + step - 1) / step;      // the same in all lanes
-    for (int r = 0; r < rounds; r += U) {
-        uint4 raw[U];
+    const int lane = threadIdx.x & 31;
+    unsigned owners = __ballot_sync(0xffffffffu, largest >= least && largest > -INFINITY);
+    while (owners) {
+        const int first = start + __ffs(owners) - 1;
+        owners &= owners - 1;
+        for (int r = 0; first + r * step < last; r += 32 * U) {
+            uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int v = first + (r + u) * step;
-            raw[u] = any && r + u < rounds && v < last ? xv[v] : make_uint4(nothing, nothing, nothing, nothing);
-        }
-        unsigned hits = 0;                                      // bit u * V + e: element e of vector u reaches the bound
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const float m = max_raw(raw[u], T());
-            if (m >= least && m > -INFINITY) {
-                float x[V];
-                unpack16<T>(raw[u], x);
-#pragma unroll
-                for (int e = 0; e < V; e++) hits |= x[e] >= least && x[e] > -INFINITY ? 1u << (u * V + e) : 0u;
+            for (int u = 0; u < U; u++) {
+                const long long v = first + (long long)(r + u * 32 + lane) * step;
+                raw[u] = v < last ? xv[v] : make_uint4(nothing, nothing, nothing, nothing);
             }
-        }
-        while (__any_sync(0xffffffffu, hits != 0)) {
-            Key key = 0;
-            if (hits) {
-                const int slot = __ffs(hits) - 1;
-                hits &= hits - 1;
-                const int at = (first + (r + slot / V) * step) * V + slot % V;
-                key = make_key(to_f32(reinterpret_cast<const T*>(xv)[at]), at + head);     // the registers cannot be indexed
+            unsigned hits = 0;                                  // bit u * V + e: element e of vector u reaches the bound
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float m = max_raw(raw[u], T());
+                if (m >= least && m > -INFINITY) {
+                    float x[V];
+                    unpack16<T>(raw[u], x);
+#pragma unroll
+                    for (int e = 0; e < V; e++) hits |= x[e] >= least && x[e] > -INFINITY ? 1u << (u * V + e) : 0u;
+                }
             }
-            top.push(key, buffer, k);
+            while (__any_sync(0xffffffffu, hits != 0)) {
+                Key key = 0;
+                if (hits) {
+                    const int slot = __ffs(hits) - 1;
+                    hits &= hits - 1;
+                    const int at = (first + (r + slot / V * 32 + lane) * step) * V + slot % V;
+                    key = make_key(to_f32(reinterpret_cast<const T*>(xv)[at]), at + head);     // the registers cannot be indexed
+                }
+                top.push(key, buffer, k);
+            }
         }
     }
 }
@@ -386,7 +390,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
         const float least = key_value((Key)__shfl_sync(0xffffffffu, sorted, q.top - 1) << 32);
         Top best;
         best.clear();
-        collect<T>(best, q.top, buffer, least, a.m, xv, v0 + tid, v1, STEP, head);
+        collect<T>(best, q.top, buffer, least, a.m, xv, v0 + tid - lane, v1, STEP, head);
         const bool hit = edge >= least && edge > -INFINITY;
         if (__any_sync(0xffffffffu, hit)) best.push(hit ? make_key(edge, edge_at) : 0, buffer, q.top);
         best.finish(buffer, q.top);
