@@ -543,88 +543,114 @@ def learn_step_weight_decay_momentum(W, momentum, dW, learnrate, momentum_weight
 
 
 # ---- operators of a token model --------------------------------------------------------------------------------
+# These are called once per generated token too, so the checks look at every property once and allocate nothing.
 
-def _float_types():
-    torch = _torch()
-    return {torch.float32: _capi.T_F32, torch.float16: _capi.T_F16, torch.bfloat16: _capi.T_BF16}
+_FLOAT_TYPES, _TOKEN_TYPES = {}, {}
+
+
+def _float_type(dtype):
+    """CUVDIA_T_* code of a float type, None for any other."""
+    if not _FLOAT_TYPES:
+        torch = _torch()
+        _TOKEN_TYPES.update({torch.int32: _capi.T_I32, torch.int64: _capi.T_I64})
+        _FLOAT_TYPES.update({torch.float32: _capi.T_F32, torch.float16: _capi.T_F16, torch.bfloat16: _capi.T_BF16})
+    return _FLOAT_TYPES.get(dtype)
 
 
 def _invalid(message):
     raise CuvDiaError(_capi.ERR_INVALID, message)
 
 
-def _matrix(t, name, device=None, shape=None, dtype=None):
-    """Leading dimension of a column-major matrix in one of the float types; ``device``, ``shape``, ``dtype``: what it
-    has to share with the call's other operands."""
-    if not (isinstance(t, _torch().Tensor) and t.dim() == 2 and t.dtype in _float_types()):
-        _invalid(name + " must be a 2-D tensor of float32, float16 or bfloat16")
+def _matrix(t, name, like=None, shape=None, dtype=None):
+    """(leading dimension, type code) of a column-major matrix in one of the float types; ``like``: a tensor whose device it
+    has to share; ``shape``, ``dtype``: what it has to have."""
+    if not isinstance(t, _torch().Tensor) or t.dim() != 2:
+        _invalid(name + " must be a 2-D tensor")
+    code = _float_type(t.dtype)
+    if code is None:
+        _invalid(name + " must be a tensor of float32, float16 or bfloat16")
     if dtype is not None and t.dtype != dtype:
         _invalid("%s has type %s, not %s" % (name, t.dtype, dtype))
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        _invalid("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
     rows, cols = t.shape
-    if rows > 1 and t.stride(0) != 1:
+    if shape is not None and (rows != shape[0] or cols != shape[1]):
+        _invalid("%s has shape %s, not %s" % (name, (rows, cols), tuple(shape)))
+    between, ld = t.stride()
+    if rows > 1 and between != 1:
         _invalid(name + " must be column-major (stride(0) == 1)")
-    ld = t.stride(1) if cols > 1 else max(rows, 1)
+    if cols <= 1:
+        ld = max(rows, 1)
     if rows < 1 or ld < rows:
         _invalid(name + " has no rows or overlapping columns")
-    if max(ld, cols) > 2147483647:
+    if ld > 2147483647 or cols > 2147483647:
         _invalid(name + " has a dimension beyond 2^31 - 1")
-    _on_device(t, name, device)
-    return int(ld)
+    _on_device(t, name, like)
+    return ld, code
 
 
-def _vector(t, name, size, device):
+def _vector(t, name, size, like):
     """A packed float32 vector."""
-    if not (isinstance(t, _torch().Tensor) and t.dim() == 1 and t.dtype == _torch().float32 and t.is_contiguous()):
+    if not isinstance(t, _torch().Tensor) or t.dim() != 1 or t.dtype != _torch().float32 or not t.is_contiguous():
         _invalid(name + " must be a contiguous 1-D float32 tensor")
-    if t.numel() != size:
-        _invalid("%s has %d elements, not %d" % (name, t.numel(), size))
-    _on_device(t, name, device)
+    if t.shape[0] != size:
+        _invalid("%s has %d elements, not %d" % (name, t.shape[0], size))
+    _on_device(t, name, like)
 
 
-def _token_type(t, ncols, device):
-    torch = _torch()
-    if not (isinstance(t, torch.Tensor) and t.dim() == 1 and t.dtype in (torch.int32, torch.int64) and t.is_contiguous()):
+def _token_type(t, ncols, like):
+    code = _TOKEN_TYPES.get(t.dtype) if isinstance(t, _torch().Tensor) and t.dim() == 1 and t.is_contiguous() else None
+    if code is None:
         _invalid("tokens must be a contiguous 1-D int32 or int64 tensor")
-    if t.numel() != ncols:
-        _invalid("tokens has %d elements, not one per column (%d)" % (t.numel(), ncols))
-    _on_device(t, "tokens", device)
-    return _capi.T_I32 if t.dtype == torch.int32 else _capi.T_I64
+    if t.shape[0] != ncols:
+        _invalid("tokens has %d elements, not one per column (%d)" % (t.shape[0], ncols))
+    _on_device(t, "tokens", like)
+    return code
 
 
-def _on_device(t, name, device):
+def _on_device(t, name, like):
     if not t.is_cuda:
         _invalid(name + " must be a CUDA tensor")
-    if device is not None and t.device != device:
-        _invalid("%s is on %s, not on %s" % (name, t.device, device))
+    if like is not None and t.get_device() != like.get_device():
+        _invalid("%s is on %s, not on %s" % (name, t.device, like.device))
 
 
-def _call(device, name, *args):
-    """Calls an entry point with ``device`` current and on its current stream."""
+def _address(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _raw_stream(index):
+    """The current stream of a device as an integer (the Stream object of :func:`_stream` costs as much as the whole call)."""
     torch = _torch()
-    if torch.cuda.current_device() == device.index:
-        _capi.check(getattr(_capi.lib(), name)(*args, _stream()))
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _call(like, name, *args):
+    """Calls an entry point with the device of the tensor ``like`` current and on its current stream."""
+    cuda, index = _torch().cuda, like.get_device()
+    entry = getattr(_capi.lib(), name)
+    if cuda.current_device() == index:
+        code = entry(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            _capi.check(getattr(_capi.lib(), name)(*args, _stream()))
+        with cuda.device(index):
+            code = entry(*args, _raw_stream(index))
+    if code:
+        _capi.check(code)
 
 
 def embedding(dst, table, tokens, scale=1.0):
     """dst[:, j] = scale * table[:, tokens[j]]; a column of zeros where the token lies outside the table (padding).
     ``table`` is units x vocab, ``dst`` units x ncols, column-major, both float32, float16 or bfloat16; ``tokens`` int32 or
     int64, one per column."""
-    ldt = _matrix(table, "table")
-    dev, (units, vocab) = table.device, table.shape
-    if not isinstance(dst, _torch().Tensor) or dst.dim() != 2:
-        _invalid("dst must be a 2-D tensor")
-    ncols = dst.shape[1]
-    ldd = _matrix(dst, "dst", dev, (units, ncols), table.dtype)
-    tt = _token_type(tokens, ncols, dev)
-    if ncols == 0:
-        return dst
-    _call(dev, "cuvdia_embedding", _ptr(dst), ldd, _ptr(table), ldt, _float_types()[table.dtype], units, vocab, _ptr(tokens),
-          tt, ncols, float(scale))
+    ldt, code = _matrix(table, "table")
+    units, vocab = table.shape
+    ldd, _ = _matrix(dst, "dst", table, None, table.dtype)
+    rows, ncols = dst.shape
+    if rows != units:
+        _invalid("dst has %d rows, the table %d" % (rows, units))
+    tt = _token_type(tokens, ncols, table)
+    if ncols:
+        _call(table, "cuvdia_embedding", dst.data_ptr(), ldd, table.data_ptr(), ldt, code, units, vocab, tokens.data_ptr(), tt,
+              ncols, scale)
     return dst
 
 
@@ -634,19 +660,20 @@ def embedding_grad(dtable, tokens, dout, factNew=1.0, factOld=0.0):
     ``factOld=0`` writes zeros into the columns of tokens that do not occur; ``factOld=1`` leaves those alone.  ``dtable`` has
     the type of ``dout`` or float32."""
     torch = _torch()
-    ldo = _matrix(dout, "dout")
-    dev, (units, ncols) = dout.device, dout.shape
-    if not isinstance(dtable, torch.Tensor) or dtable.dim() != 2 or dtable.dtype not in (dout.dtype, torch.float32):
-        _invalid("dtable must be a 2-D tensor of dout's type or float32")
-    vocab = dtable.shape[1]
-    ldt = _matrix(dtable, "dtable", dev, (units, vocab))
-    tt = _token_type(tokens, ncols, dev)
+    ldo, code = _matrix(dout, "dout")
+    units, ncols = dout.shape
+    ldt, grad_code = _matrix(dtable, "dtable", dout)
+    rows, vocab = dtable.shape
+    if rows != units:
+        _invalid("dtable has %d rows, dout %d" % (rows, units))
+    if grad_code != code and grad_code != _capi.T_F32:
+        _invalid("dtable must have dout's type or float32")
+    tt = _token_type(tokens, ncols, dout)
     need = ctypes.c_longlong()
     _capi.check(_capi.lib().cuvdia_embedding_grad_workspace(units, vocab, ncols, ctypes.byref(need)))
-    work = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    types = _float_types()
-    _call(dev, "cuvdia_embedding_grad", _ptr(dtable), ldt, types[dtable.dtype], _ptr(dout), ldo, types[dout.dtype], units, vocab,
-          _ptr(tokens), tt, ncols, float(factNew), float(factOld), _ptr(work), need.value)
+    work = torch.empty(need.value, dtype=torch.uint8, device=dout.device)
+    _call(dout, "cuvdia_embedding_grad", dtable.data_ptr(), ldt, grad_code, dout.data_ptr(), ldo, code, units, vocab,
+          tokens.data_ptr(), tt, ncols, factNew, factOld, work.data_ptr(), need.value)
     return dtable
 
 
@@ -654,15 +681,14 @@ def dropout(dst, src, p, seed, step=0, col0=0, which=0, residual=None):
     """dst = (u >= p ? src / (1 - p) : 0) [+ residual], u the uniform number :func:`fill_rnd_uniform` gives for the same
     (seed, step, col0, which): no mask is stored, :func:`dropout_grad` draws the same one again.  float32, float16 or
     bfloat16, all of one type; ``dst`` may be ``src`` or ``residual``."""
-    lds = _matrix(src, "src")
-    dev, (rows, ncols) = src.device, src.shape
-    ldd = _matrix(dst, "dst", dev, src.shape, src.dtype)
-    ldr = _matrix(residual, "residual", dev, src.shape, src.dtype) if residual is not None else 0
-    if ncols == 0:
-        return dst
-    d = _capi.Draw(int(seed), int(step), int(col0))
-    _call(dev, "cuvdia_dropout", _ptr(dst), ldd, _ptr(src), lds, _ptr(residual), ldr, _float_types()[src.dtype], rows, ncols,
-          float(p), ctypes.byref(d), int(which))
+    lds, code = _matrix(src, "src")
+    shape, dtype = src.shape, src.dtype
+    ldd, _ = _matrix(dst, "dst", src, shape, dtype)
+    ldr = _matrix(residual, "residual", src, shape, dtype)[0] if residual is not None else 0
+    rows, ncols = shape
+    if ncols:
+        _call(src, "cuvdia_dropout", dst.data_ptr(), ldd, src.data_ptr(), lds, _address(residual), ldr, code, rows, ncols, p,
+              ctypes.byref(_capi.Draw(seed, step, col0)), which)
     return dst
 
 
@@ -682,23 +708,24 @@ def token_logprob(logits, tokens=None, scale=1.0, entropy=False, top=0):
     ``top_index`` of shape (top, ncols).  Returns a :class:`TokenLogprob` of new float32 (int32) tensors, None for what
     was not asked for.  A logit of -inf is a forbidden token."""
     torch = _torch()
-    ld = _matrix(logits, "logits")
-    dev, (vocab, ncols) = logits.device, logits.shape
-    tt = _token_type(tokens, ncols, dev) if tokens is not None else 0
-    top = int(top)
+    ld, code = _matrix(logits, "logits")
+    vocab, ncols = logits.shape
+    tt = _token_type(tokens, ncols, logits) if tokens is not None else 0
     if not 0 <= top <= 32:
         _invalid("0 <= top <= 32")
-    # one allocation for all results
-    n = ncols * (1 + (tokens is not None) + bool(entropy))
-    out = torch.empty(n + ncols * top, dtype=torch.float32, device=dev)
-    lse = out[:ncols]
-    logp = out[ncols:2 * ncols] if tokens is not None else None
-    ent = out[n - ncols:n] if entropy else None
-    top_logp = out[n:].view(ncols, top).t() if top else None
-    top_index = torch.empty((ncols, top), dtype=torch.int32, device=dev).t() if top else None
+    device = logits.device
+    # lse, logp and entropy are rows of one allocation
+    rows = iter(torch.empty((1 + (tokens is not None) + bool(entropy), ncols), dtype=torch.float32, device=device).unbind())
+    lse = next(rows)
+    logp = next(rows) if tokens is not None else None
+    ent = next(rows) if entropy else None
+    top_logp = top_index = None
+    if top:
+        top_logp = torch.empty_strided((top, ncols), (1, top), dtype=torch.float32, device=device)
+        top_index = torch.empty_strided((top, ncols), (1, top), dtype=torch.int32, device=device)
     if ncols:
-        _call(dev, "cuvdia_token_logprob", _ptr(logits), ld, _float_types()[logits.dtype], vocab, ncols, _ptr(tokens), tt,
-              float(scale), _ptr(logp), _ptr(lse), _ptr(ent), top, _ptr(top_logp), _ptr(top_index))
+        _call(logits, "cuvdia_token_logprob", logits.data_ptr(), ld, code, vocab, ncols, _address(tokens), tt, scale,
+              _address(logp), lse.data_ptr(), _address(ent), top, _address(top_logp), _address(top_index))
     return TokenLogprob(logp, lse, ent, top_logp, top_index)
 
 
@@ -706,16 +733,15 @@ def token_logprob_grad(dlogits, logits, lse, tokens=None, dlogp=None, entropy=No
     """dlogits[v, j] = scale * (dlogp[j]*([v == tokens[j]] - p_v) - dentropy[j]*p_v*(log p_v + entropy[j])): the gradient of a
     loss through :func:`token_logprob`'s ``logp`` (``tokens`` and ``dlogp``) and ``entropy`` (``entropy`` and ``dentropy``);
     ``lse``, ``entropy`` are its results, ``scale`` its scale.  ``dlogits`` has the type of ``logits`` and may be ``logits``."""
-    ld = _matrix(logits, "logits")
-    dev, (vocab, ncols) = logits.device, logits.shape
-    ldd = _matrix(dlogits, "dlogits", dev, logits.shape, logits.dtype)
-    _vector(lse, "lse", ncols, dev)
-    tt = _token_type(tokens, ncols, dev) if tokens is not None else 0
+    ld, code = _matrix(logits, "logits")
+    vocab, ncols = logits.shape
+    ldd, _ = _matrix(dlogits, "dlogits", logits, (vocab, ncols), logits.dtype)
+    _vector(lse, "lse", ncols, logits)
+    tt = _token_type(tokens, ncols, logits) if tokens is not None else 0
     for t, name in ((dlogp, "dlogp"), (entropy, "entropy"), (dentropy, "dentropy")):
         if t is not None:
-            _vector(t, name, ncols, dev)
-    if ncols == 0:
-        return dlogits
-    _call(dev, "cuvdia_token_logprob_grad", _ptr(dlogits), ldd, _ptr(logits), ld, _float_types()[logits.dtype], vocab, ncols,
-          _ptr(tokens), tt, float(scale), _ptr(lse), _ptr(dlogp), _ptr(entropy), _ptr(dentropy))
+            _vector(t, name, ncols, logits)
+    if ncols:
+        _call(logits, "cuvdia_token_logprob_grad", dlogits.data_ptr(), ldd, logits.data_ptr(), ld, code, vocab, ncols,
+              _address(tokens), tt, scale, lse.data_ptr(), _address(dlogp), _address(entropy), _address(dentropy))
     return dlogits

@@ -124,7 +124,8 @@ __device__ __forceinline__ K merge_warps(K mine, K (*lists)[32], int n) {
 // The best 32 of a descending list and 32 candidates in any order.  Called, not inlined: it is rare and long, and copies of it
 // cost more in instruction fetches than the calls.
 __device__ __noinline__ Key absorb32(Key list, Key batch) { return merge_desc(list, sort_desc(batch)); }
-__device__ __noinline__ unsigned sort_maxima(unsigned k) { return sort_desc(k); }
+__device__ __noinline__ unsigned sort_upper(unsigned k) { return sort_desc(k); }
+__device__ __noinline__ Key sort_keys(Key k) { return sort_desc(k); }
 
 // A warp's best candidates: a descending list (one a lane), and up to 63 more in shared memory that wait to be sorted in,
 // 32 at a time.  `bar` is the k-th best of the list: what a new one has to beat.
@@ -163,9 +164,10 @@ struct Top {
 // all: only the few threads whose largest logit reaches it own any, and what is read again lies in L2.  The warp goes through
 // the vectors of one such thread after the other, 64 at a time.  xv: the column's whole vectors; the warp's own are
 // start + lane, start + lane + step, .. below last.
-template <class T>
-__device__ __forceinline__ void collect(Top& top, int k, Key* buffer, float least, float largest, const uint4* xv, int start,
-                                        int last, int step, int head) {
+// take(key): one candidate per lane at most (0: none), called by the whole warp.
+template <class T, class F>
+__device__ __forceinline__ void collect(F&& take, float least, float largest, const uint4* xv, int start, int last, int step,
+                                        int head) {
     constexpr int V = Vec16<T>::N, U = 2;
     const unsigned nothing = minus_inf_word<T>();
     const int lane = threadIdx.x & 31;
@@ -199,7 +201,7 @@ __device__ __forceinline__ void collect(Top& top, int k, Key* buffer, float leas
                     const int at = (first + (r + slot / V * 32 + lane) * step) * V + slot % V;
                     key = make_key(to_f32(reinterpret_cast<const T*>(xv)[at]), at + head);     // the registers cannot be indexed
                 }
-                top.push(key, buffer, k);
+                take(key);
             }
         }
     }
@@ -323,7 +325,8 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     constexpr int V = Vec16<T>::N, U = 4, WARPS = 8, STEP = TEAM;
     __shared__ Stat stats[WARPS], part_stats[WARPS];
     __shared__ Key lists[TOP ? WARPS : 1][32], part_lists[TOP ? WARPS : 1][32], buffers[TOP ? WARPS : 1][64];
-    __shared__ unsigned maxima[TOP ? WARPS : 1][32];
+    __shared__ unsigned maxima[TOP ? 32 : 1];
+    __shared__ int found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = TEAM == 256 ? blockIdx.x % (unsigned)parts : 0;
     const long long col = TEAM == 256 ? blockIdx.x / (unsigned)parts : (long long)blockIdx.x * WARPS + warp;
@@ -332,7 +335,6 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     const T* x0 = (const T*)q.logits + col * q.ld;
     const float c = q.scale * LOG2E;
     const int tid = TEAM == 256 ? threadIdx.x : lane;
-    Key* buffer = buffers[TOP ? warp : 0];
     // whole 16-byte vectors of the column, behind `head` elements and before the rest
     const int head = min(q.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)));
     const int nvec = (q.vocab - head) / V, rest = q.vocab - head - nvec * V;
@@ -378,23 +380,54 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     }
     Key list = 0;
     if (TOP) {
-        // The k-th largest of the threads' largest logits bounds the k-th best from below, and few logits reach it.
-        const unsigned own = a.m > -INFINITY ? (unsigned)(make_key(a.m, 0) >> 32) : 0;
-        unsigned sorted = sort_maxima(own);
-        if (TEAM == 256) {
-            sorted = merge_warps(sorted, maxima, WARPS);
-            if (warp == 0) maxima[0][lane] = sorted;
+        // The k-th largest of some of the threads' largest logits bounds the k-th best from below, and few logits reach it.
+        unsigned own = a.m > -INFINITY ? (unsigned)(make_key(a.m, 0) >> 32) : 0;
+        if (TEAM == 256) {                                      // the four largest of each warp
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned m = __reduce_max_sync(0xffffffffu, own);
+                const int from = __ffs(__ballot_sync(0xffffffffu, own == m)) - 1;
+                if (lane == from) own = 0;
+                if (lane == 0) maxima[warp * 4 + j] = m;
+            }
+            if (threadIdx.x == 0) found = 0;
             __syncthreads();
-            sorted = maxima[0][lane];
+            own = maxima[lane];
         }
-        const float least = key_value((Key)__shfl_sync(0xffffffffu, sorted, q.top - 1) << 32);
-        Top best;
-        best.clear();
-        collect<T>(best, q.top, buffer, least, a.m, xv, v0 + tid - lane, v1, STEP, head);
-        const bool hit = edge >= least && edge > -INFINITY;
-        if (__any_sync(0xffffffffu, hit)) best.push(hit ? make_key(edge, edge_at) : 0, buffer, q.top);
-        best.finish(buffer, q.top);
-        list = best.list;
+        const float least = key_value((Key)__shfl_sync(0xffffffffu, sort_upper(own), q.top - 1) << 32);
+        const bool at_edge = edge >= least && edge > -INFINITY;
+        // A block gathers its candidates in shared memory; a warp on its own, and a block with more of them than fit there
+        // (many ties), sorts them into lists of its warps as they come.
+        if (TEAM == 256) {
+            auto take = [&](Key key) {
+                const unsigned there = __ballot_sync(0xffffffffu, key != 0);
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&found, __popc(there));
+                at = __shfl_sync(0xffffffffu, at, 0) + __popc(there & ((1u << lane) - 1));
+                if (key != 0 && at < WARPS * 32) (&lists[0][0])[at] = key;
+            };
+            collect<T>(take, least, a.m, xv, v0 + tid - lane, v1, STEP, head);
+            if (__any_sync(0xffffffffu, at_edge)) take(at_edge ? make_key(edge, edge_at) : 0);
+            __syncthreads();
+        }
+        const int n = TEAM == 256 ? found : WARPS * 32 + 1;
+        if (n <= WARPS * 32) {
+            if (warp * 32 < n) list = sort_keys(warp * 32 + lane < n ? lists[warp][lane] : 0);
+            __syncthreads();
+            if (n > 32) list = merge_warps(list, lists, WARPS);
+        } else {
+            Top best;
+            best.clear();
+            auto take = [&](Key key) { best.push(key, buffers[warp], q.top); };
+            collect<T>(take, least, a.m, xv, v0 + tid - lane, v1, STEP, head);
+            if (__any_sync(0xffffffffu, at_edge)) take(at_edge ? make_key(edge, edge_at) : 0);
+            best.finish(buffers[warp], q.top);
+            list = best.list;
+            if (TEAM == 256) {
+                __syncthreads();
+                list = merge_warps(list, lists, WARPS);
+            }
+        }
     }
     Stat st = join_warp<ENT>(a, c);
     if (TEAM == 32) { write_column<T, ENT, TOP>(q, col, x0, st, list); return; }
@@ -407,7 +440,6 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
             st = stats[0];
             for (int w = 1; w < n; w++) st = merge(st, stats[w], c);
         }
-        if (TOP) list = merge_warps(list, lists, n);
     };
     join(WARPS);
     if (parts > 1) {
@@ -426,6 +458,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
         if (TOP) list = part_lists[min(warp, parts - 1)][lane];
         __syncthreads();
         join(parts);
+        if (TOP) list = merge_warps(list, lists, parts);
     }
     if (warp == 0) write_column<T, ENT, TOP>(q, col, x0, st, list);
 }
