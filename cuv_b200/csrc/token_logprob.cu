@@ -64,6 +64,8 @@ template <> __device__ __forceinline__ unsigned minus_inf_word<float>() { return
 template <> __device__ __forceinline__ unsigned minus_inf_word<__half>() { return 0xfc00fc00u; }
 template <> __device__ __forceinline__ unsigned minus_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
 
+constexpr int U = 4;                    // vectors a thread takes at a time: a chunk
+
 // ---- the likeliest tokens ------------------------------------------------------------------------------------------
 // A candidate is one 64-bit number that orders like (logit descending, index ascending): the larger, the better; 0 = none.
 // NaN and -inf are never candidates.
@@ -160,45 +162,86 @@ struct Top {
     }
 };
 
+// What a thread remembers of its chunks for `collect`: the vector index at which the chunk with its largest logit begins, and
+// the largest logit of its other chunks.
+struct Where { int chunk; float second; };
+
 // The candidates among a warp's vectors, looked at a second time once `least` is known, a lower bound on the k-th best logit of
-// all: only the few threads whose largest logit reaches it own any, and what is read again lies in L2.  The warp goes through
-// the vectors of one such thread after the other, 64 at a time.  xv: the column's whole vectors; the warp's own are
+// all: only the few threads whose largest logit reaches it own any, nearly always in the one chunk they remember, and what is
+// read again lies in L2.  The warp looks at the U vectors of 32 / U such chunks at once; the vectors of a thread with
+// candidates in several chunks it goes through 64 at a time.  xv: the column's whole vectors; the warp's own are
 // start + lane, start + lane + step, .. below last.
 // take(key): one candidate per lane at most (0: none), called by the whole warp.
 template <class T, class F>
-__device__ __forceinline__ void collect(F&& take, float least, float largest, const uint4* xv, int start, int last, int step,
-                                        int head) {
-    constexpr int V = Vec16<T>::N, U = 2;
+__device__ __forceinline__ void collect(F&& take, float least, float largest, const Where& w, const uint4* xv, int start, int last,
+                                        int step, int head) {
+    constexpr int V = Vec16<T>::N, G = 4, W = 2;
     const unsigned nothing = minus_inf_word<T>();
     const int lane = threadIdx.x & 31;
-    unsigned owners = __ballot_sync(0xffffffffu, largest >= least && largest > -INFINITY);
+    const bool any = largest >= least && largest > -INFINITY;
+    unsigned owners = __ballot_sync(0xffffffffu, any && !(w.second >= least));
     while (owners) {
-        const int first = start + __ffs(owners) - 1;
-        owners &= owners - 1;
-        for (int r = 0; first + r * step < last; r += 32 * U) {
-            uint4 raw[U];
+        int v = last;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const long long v = first + (long long)(r + u * 32 + lane) * step;
-                raw[u] = v < last ? xv[v] : make_uint4(nothing, nothing, nothing, nothing);
-            }
-            unsigned hits = 0;                                  // bit u * V + e: element e of vector u reaches the bound
+        for (int g = 0; g < 32 / U; g++) {
+            const int from = owners ? __ffs(owners) - 1 : 0;
+            const int chunk = __shfl_sync(0xffffffffu, w.chunk, from);
+            if (owners && lane / U == g) v = chunk + from + lane % U * step;
+            owners &= owners - 1;
+        }
+        const uint4 raw = v < last ? xv[v] : make_uint4(nothing, nothing, nothing, nothing);
+        float x[V];
+        unpack16<T>(raw, x);
+        unsigned hits = 0;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const float m = max_raw(raw[u], T());
-                if (m >= least && m > -INFINITY) {
-                    float x[V];
-                    unpack16<T>(raw[u], x);
+        for (int e = 0; e < V; e++) hits |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0u;
+        while (__any_sync(0xffffffffu, hits != 0)) {
+            Key key = 0;
 #pragma unroll
-                    for (int e = 0; e < V; e++) hits |= x[e] >= least && x[e] > -INFINITY ? 1u << (u * V + e) : 0u;
+            for (int e = V - 1; e >= 0; e--) if (hits >> e & 1) key = make_key(x[e], v * V + e + head);
+            hits &= hits - 1;
+            take(key);
+        }
+    }
+    owners = __ballot_sync(0xffffffffu, any && w.second >= least);
+    while (owners) {
+        int first[G];                                           // four threads' vectors are in flight at a time
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            first[g] = owners ? start + __ffs(owners) - 1 : last;
+            owners &= owners - 1;
+        }
+        for (int r = 0; first[0] + r * step < last; r += 32 * W) {
+            uint4 raw[G][W];
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    const long long v = first[g] + (long long)(r + u * 32 + lane) * step;
+                    raw[g][u] = v < last ? xv[v] : make_uint4(nothing, nothing, nothing, nothing);
                 }
-            }
+            unsigned long long hits = 0;                        // bit (g * W + u) * V + e: element e of vector u of thread g
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    const float m = max_raw(raw[g][u], T());
+                    if (m >= least && m > -INFINITY) {
+                        float x[V];
+                        unpack16<T>(raw[g][u], x);
+                        unsigned h = 0;
+#pragma unroll
+                        for (int e = 0; e < V; e++) h |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0u;
+                        hits |= (unsigned long long)h << ((g * W + u) * V);
+                    }
+                }
             while (__any_sync(0xffffffffu, hits != 0)) {
                 Key key = 0;
                 if (hits) {
-                    const int slot = __ffs(hits) - 1;
+                    const int slot = __ffsll(hits) - 1, g = slot / (W * V), u = slot / V % W;
                     hits &= hits - 1;
-                    const int at = (first + (r + slot / V * 32 + lane) * step) * V + slot % V;
+                    const int f = g == 0 ? first[0] : g == 1 ? first[1] : g == 2 ? first[2] : first[3];
+                    const int at = (f + (r + u * 32 + lane) * step) * V + slot % V;
                     key = make_key(to_f32(reinterpret_cast<const T*>(xv)[at]), at + head);     // the registers cannot be indexed
                 }
                 take(key);
@@ -211,62 +254,104 @@ __device__ __forceinline__ void collect(F&& take, float least, float largest, co
 // The sums of a thread as pairs, so that two elements share an instruction.
 struct Sums { float m; float2 s, t; };
 
-// The 32 threads' sums as one, in all lanes: relative to the warp's maximum first, so that only one rescaling each is needed.
-template <bool ENT>
-__device__ __forceinline__ Stat join_warp(Sums& a, float c) {
-    float m;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(a.m));
-    Stat r = {a.m, a.s.x + a.s.y, ENT ? a.t.x + a.t.y : 0.f};
-    rescale(r, m, c);
+// The sums of LANES neighbouring lanes as one, in all of them: relative to their maximum first, so that only one rescaling each
+// is needed.
+template <bool ENT, int LANES>
+__device__ __forceinline__ Stat join_lanes(Stat r, float c) {
+    float m = r.m;
+    if (LANES == 32) {
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(r.m));
+    } else {
 #pragma unroll
-    for (int s = 16; s > 0; s /= 2) {
+        for (int s = LANES / 2; s > 0; s /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+    }
+    if (r.m != m) rescale(r, m, c);
+#pragma unroll
+    for (int s = LANES / 2; s > 0; s /= 2) {
         r.s += __shfl_xor_sync(0xffffffffu, r.s, s);
         if (ENT) r.t += __shfl_xor_sync(0xffffffffu, r.t, s);
     }
     return r;
 }
 
-// Adds U vectors to a thread's sums, two elements an instruction.  An exponent of -inf (a forbidden token) times its power of
-// zero is NaN; such a chunk is summed once more with its exponents cut (see LEAST), the others need no test per element.
-template <class T, bool ENT, int U>
-__device__ __forceinline__ void add_chunk(Sums& a, float m, const uint4 (&raw)[U], float c) {
-    constexpr int V = Vec16<T>::N;
-    if (m > a.m) {
-        if (a.m != -INFINITY) {
-            const float by = (a.m - m) * c, f = exp2_approx(by), cut = fmaxf(by, LEAST);
-            if (ENT) { a.t.x = f * fmaf(a.s.x, cut, a.t.x); a.t.y = f * fmaf(a.s.y, cut, a.t.y); }
-            a.s.x *= f; a.s.y *= f;
-        }
-        a.m = m;
+// The vectors of a column on their way through shared memory: a thread copies its own vectors in asynchronously, some chunks
+// ahead, and reads back what it copied itself, so that no barrier is involved and vectors in flight hold no registers.
+
+__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+template <class T>
+__device__ __forceinline__ float max_chunk(const uint4* v, int step) {
+    float m = max_raw(v[0], T());
+#pragma unroll
+    for (int u = 1; u < U; u++) m = fmaxf(m, max_raw(v[u * step], T()));
+    return m;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void raise(Sums& a, float m, float c) {
+    if (!(m > a.m)) return;
+    if (a.m != -INFINITY) {
+        const float by = (a.m - m) * c, f = exp2_approx(by), cut = fmaxf(by, LEAST);
+        if (ENT) { a.t.x = f * fmaf(a.s.x, cut, a.t.x); a.t.y = f * fmaf(a.s.y, cut, a.t.y); }
+        a.s.x *= f; a.s.y *= f;
     }
-    const float m0 = shift(a.m);
+    a.m = m;
+}
+
+// Adds a chunk, the U vectors v, v + step, .., to a thread's sums, two elements an instruction.  The sums may be relative to any
+// logit that keeps the powers finite, so the maximum is only looked for in a thread's first chunk (MAX: in every chunk, for
+// callers that want the maximum itself).  A chunk whose sums come out beyond 1e30 or NaN - a logit far above the first chunk's,
+// or an exponent of -inf (a forbidden token) times its power of zero - is summed once more relative to its maximum and with its
+// exponents cut (see LEAST); the others need no test per element.
+template <class T, bool ENT, bool MAX>
+__device__ __forceinline__ void add_chunk(Sums& a, const uint4* v, int step, float c, Where& w, int at) {
+    constexpr int V = Vec16<T>::N;
+    if (MAX) {
+        const float m = max_chunk<T>(v, step), before = a.m;
+        if (m > before) w.chunk = at;
+        w.second = fmaxf(w.second, fminf(m, before));
+        raise<ENT>(a, m, c);
+    } else if (a.m == -INFINITY) {
+        raise<ENT>(a, max_chunk<T>(v, step), c);
+    }
+    float m0 = shift(a.m);
     const float2 minus = make_float2(-m0, -m0), by = make_float2(c, c);
-    float2 t = make_float2(0.f, 0.f);
+    float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float x[V];
-        unpack16<T>(raw[u], x);
+        unpack16<T>(v[u * step], x);
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
             const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), minus), by);
             const float2 p = make_float2(exp2_approx(d.x), exp2_approx(d.y));
-            a.s = __fadd2_rn(a.s, p);
+            s = __fadd2_rn(s, p);
             if (ENT) t = __ffma2_rn(p, d, t);
         }
     }
-    if (ENT) {
-        if (t.x + t.y != t.x + t.y) {
-            t = make_float2(0.f, 0.f);
+    if (!(fabsf(ENT ? t.x + t.y : s.x + s.y) < 1e30f)) {
+        if (!MAX) raise<ENT>(a, max_chunk<T>(v, step), c);
+        m0 = shift(a.m);
+        s = t = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int u = 0; u < U; u++) {
+            float x[V];
+            unpack16<T>(v[u * step], x);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                float x[V];
-                unpack16<T>(raw[u], x);
-#pragma unroll
-                for (int e = 0; e < V; e++) { const float d = (x[e] - m0) * c; t.x = fmaf(exp2_approx(d), fmaxf(d, LEAST), t.x); }
+            for (int e = 0; e < V; e++) {
+                const float d = (x[e] - m0) * c, p = exp2_approx(d);
+                s.x += p;
+                if (ENT) t.x = fmaf(p, fmaxf(d, LEAST), t.x);
             }
         }
-        a.t.x += t.x; a.t.y += t.y;
     }
+    a.s = __fadd2_rn(a.s, s);
+    if (ENT) a.t = __fadd2_rn(a.t, t);
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -293,21 +378,18 @@ struct LogprobArgs {
     float* top_logp; int* top_index;
 };
 
-// The results of a column from its statistics and its descending list: one warp.
+// The results of a column from its statistics and its descending list: one warp.  given: the column's token is one of the
+// vocabulary; given_logit is its logit then.
 template <class T, bool ENT, bool TOP>
-__device__ __forceinline__ void write_column(const LogprobArgs& q, long long col, const T* x0, const Stat& a, Key list) {
+__device__ __forceinline__ void write_column(const LogprobArgs& q, long long col, bool given, float given_logit, const Stat& a,
+                                             Key list) {
     const int lane = threadIdx.x & 31;
     const bool none = a.m == -INFINITY && a.s == 0.f;
     const float m0 = shift(a.m), l2s = log2f(a.s);
     if (lane == 0) {
         if (q.lse) q.lse[col] = fmaf(m0, q.scale, l2s * LN2);
         if (ENT) { const float h = (l2s - a.t / a.s) * LN2; q.entropy[col] = none || h < 0.f ? 0.f : h; }
-        if (q.logp) {
-            const long long t = q.tokens[col];
-            float r = 0.f;
-            if (t >= 0 && t < q.vocab) r = none ? -INFINITY : fmaf(to_f32(x0[t]) - m0, q.scale, -l2s * LN2);
-            q.logp[col] = r;
-        }
+        if (q.logp) q.logp[col] = !given ? 0.f : none ? -INFINITY : fmaf(given_logit - m0, q.scale, -l2s * LN2);
     }
     if (TOP && lane < q.top) {
         q.top_logp[col * q.top + lane] = list == 0 ? -INFINITY : fmaf(key_value(list) - m0, q.scale, -l2s * LN2);
@@ -315,60 +397,76 @@ __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col
     }
 }
 
-// TEAM threads share a column's part: a whole block of 256, or a warp (eight columns a block) where a column is so short
+// TEAM threads share a column's part: a whole block, or a warp (eight columns a block of 256) where a column is so short
 // that a block's joins would cost more than its elements.  A cluster of `parts` blocks shares a column where the columns
 // alone are too few to fill the GPU: its blocks leave their sums and lists in the first block's shared memory, which joins
 // them, so that there is one launch and no scratch memory.
 template <class T, bool ENT, bool TOP, int TEAM>
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM, TEAM == 128 ? 8 : 4)
 token_logprob_kernel(const LogprobArgs q, int parts) {
-    constexpr int V = Vec16<T>::N, U = 4, WARPS = 8, STEP = TEAM;
-    __shared__ Stat stats[WARPS], part_stats[WARPS];
-    __shared__ Key lists[TOP ? WARPS : 1][32], part_lists[TOP ? WARPS : 1][32], buffers[TOP ? WARPS : 1][64];
+    constexpr int V = Vec16<T>::N, THREADS = TEAM == 32 ? 256 : TEAM, WARPS = TEAM == 32 ? 8 : TEAM / 32, STEP = TEAM;
+    constexpr int STAGES = TEAM == 128 && !TOP ? 3 : 2;          // three would not leave room for a list's arrays in as many blocks
+    constexpr bool BLOCK = TEAM != 32;
+    __shared__ uint4 ring[STAGES * U * THREADS];
+    __shared__ Stat stats[WARPS], part_stats[8];
+    __shared__ Key lists[TOP ? WARPS : 1][32], part_lists[TOP ? 8 : 1][32], buffers[TOP ? WARPS : 1][64];
     __shared__ unsigned maxima[TOP ? 32 : 1];
     __shared__ int found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int part = TEAM == 256 ? blockIdx.x % (unsigned)parts : 0;
-    const long long col = TEAM == 256 ? blockIdx.x / (unsigned)parts : (long long)blockIdx.x * WARPS + warp;
-    if (TEAM == 256 && parts > 1) cluster_arrive();             // waited for before the first remote store: all blocks run then
+    const int part = BLOCK ? blockIdx.x % (unsigned)parts : 0;
+    const long long col = BLOCK ? blockIdx.x / (unsigned)parts : (long long)blockIdx.x * WARPS + warp;
+    if (BLOCK && parts > 1) cluster_arrive();             // waited for before the first remote store: all blocks run then
     if (col >= q.ncols) return;
     const T* x0 = (const T*)q.logits + col * q.ld;
     const float c = q.scale * LOG2E;
-    const int tid = TEAM == 256 ? threadIdx.x : lane;
+    const int tid = BLOCK ? threadIdx.x : lane;
     // whole 16-byte vectors of the column, behind `head` elements and before the rest
     const int head = min(q.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)));
     const int nvec = (q.vocab - head) / V, rest = q.vocab - head - nvec * V;
     const uint4* xv = reinterpret_cast<const uint4*>(x0 + head);
     const int v0 = (int)((long long)nvec * part / parts), v1 = (int)((long long)nvec * (part + 1) / parts);
     Sums a = {-INFINITY, {0.f, 0.f}, {0.f, 0.f}};
+    Where where = {0, -INFINITY};
+    // the given token's logit, fetched here so that it need not be waited for at the end
+    bool given = false;
+    float given_logit = 0.f;
+    if (q.logp && lane == 0 && part == 0 && (!BLOCK || warp == 0)) {
+        const long long t = q.tokens[col];
+        given = t >= 0 && t < q.vocab;
+        if (given) given_logit = to_f32(x0[t]);
+    }
     const unsigned nothing = minus_inf_word<T>();
-    uint4 next[U];
-    const uint4* from = xv + v0 + tid;                          // the chunk being fetched
-    auto fetch = [&](int i) {
-        if (i + STEP * U <= v1) {
+    uint4* mine = ring + threadIdx.x;                            // [stage][u][thread]
+    const uint4* from = xv + v0 + tid;                          // the chunk to fetch next
+    int ahead = v0, stage = 0;
+    auto fetch = [&](int to) {
+        uint4* slot = mine + to * (U * THREADS);
+        if (ahead + STEP * U <= v1) {
 #pragma unroll
-            for (int u = 0; u < U; u++) next[u] = __ldg(from + u * STEP);
-        } else {
+            for (int u = 0; u < U; u++) copy_async(slot + u * THREADS, from + u * STEP);
+        } else if (ahead < v1) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                next[u] = i + u * STEP + tid < v1 ? __ldg(from + u * STEP) : make_uint4(nothing, nothing, nothing, nothing);
+            for (int u = 0; u < U; u++) {
+                if (ahead + u * STEP + tid < v1) copy_async(slot + u * THREADS, from + u * STEP);
+                else slot[u * THREADS] = make_uint4(nothing, nothing, nothing, nothing);
+            }
         }
+        copies_commit();
+        ahead += STEP * U;
         from += STEP * U;
     };
-    fetch(v0);
+#pragma unroll
+    for (int k = 0; k < STAGES; k++) fetch(k);
     for (int i = v0; i < v1; i += STEP * U) {
-        uint4 raw[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = next[u];
-        if (i + STEP * U < v1) fetch(i + STEP * U);
-        float m = max_raw(raw[0], T());
-#pragma unroll
-        for (int u = 1; u < U; u++) m = fmaxf(m, max_raw(raw[u], T()));
-        add_chunk<T, ENT, U>(a, m, raw, c);
+        copies_wait<STAGES - 1>();
+        add_chunk<T, ENT, TOP>(a, mine + stage * (U * THREADS), THREADS, c, where, i + tid - lane);
+        fetch(stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
+    const float largest = a.m;
     float edge = -INFINITY;                                     // of the ends: one element a lane at most
     int edge_at = -1;
-    if (part == 0 && (TEAM == 32 || warp == 0) && head + rest > 0) {       // the ends, element by element
+    if (part == 0 && (!BLOCK || warp == 0) && head + rest > 0) {       // the ends, element by element
         edge_at = lane < head ? lane : lane >= 16 && lane - 16 < rest ? head + nvec * V + lane - 16 : -1;
         edge = edge_at >= 0 ? to_f32(x0[edge_at]) : -INFINITY;
         Stat b = {fmaxf(edge, -INFINITY), 0.f, 0.f};            // NaN: leaves the maximum to the others
@@ -382,13 +480,12 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     if (TOP) {
         // The k-th largest of some of the threads' largest logits bounds the k-th best from below, and few logits reach it.
         unsigned own = a.m > -INFINITY ? (unsigned)(make_key(a.m, 0) >> 32) : 0;
-        if (TEAM == 256) {                                      // the four largest of each warp
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
+        if (BLOCK) {                                            // 32 of them, the same number from each warp
+            for (int j = 0; j < 32 / WARPS; j++) {
                 const unsigned m = __reduce_max_sync(0xffffffffu, own);
                 const int from = __ffs(__ballot_sync(0xffffffffu, own == m)) - 1;
                 if (lane == from) own = 0;
-                if (lane == 0) maxima[warp * 4 + j] = m;
+                if (lane == 0) maxima[warp * (32 / WARPS) + j] = m;
             }
             if (threadIdx.x == 0) found = 0;
             __syncthreads();
@@ -398,7 +495,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
         const bool at_edge = edge >= least && edge > -INFINITY;
         // A block gathers its candidates in shared memory; a warp on its own, and a block with more of them than fit there
         // (many ties), sorts them into lists of its warps as they come.
-        if (TEAM == 256) {
+        if (BLOCK) {
             auto take = [&](Key key) {
                 const unsigned there = __ballot_sync(0xffffffffu, key != 0);
                 int at = 0;
@@ -406,11 +503,11 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
                 at = __shfl_sync(0xffffffffu, at, 0) + __popc(there & ((1u << lane) - 1));
                 if (key != 0 && at < WARPS * 32) (&lists[0][0])[at] = key;
             };
-            collect<T>(take, least, a.m, xv, v0 + tid - lane, v1, STEP, head);
+            collect<T>(take, least, largest, where, xv, v0 + tid - lane, v1, STEP, head);
             if (__any_sync(0xffffffffu, at_edge)) take(at_edge ? make_key(edge, edge_at) : 0);
             __syncthreads();
         }
-        const int n = TEAM == 256 ? found : WARPS * 32 + 1;
+        const int n = BLOCK ? found : WARPS * 32 + 1;
         if (n <= WARPS * 32) {
             if (warp * 32 < n) list = sort_keys(warp * 32 + lane < n ? lists[warp][lane] : 0);
             __syncthreads();
@@ -419,29 +516,22 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
             Top best;
             best.clear();
             auto take = [&](Key key) { best.push(key, buffers[warp], q.top); };
-            collect<T>(take, least, a.m, xv, v0 + tid - lane, v1, STEP, head);
+            collect<T>(take, least, largest, where, xv, v0 + tid - lane, v1, STEP, head);
             if (__any_sync(0xffffffffu, at_edge)) take(at_edge ? make_key(edge, edge_at) : 0);
             best.finish(buffers[warp], q.top);
             list = best.list;
-            if (TEAM == 256) {
+            if (BLOCK) {
                 __syncthreads();
                 list = merge_warps(list, lists, WARPS);
             }
         }
     }
-    Stat st = join_warp<ENT>(a, c);
-    if (TEAM == 32) { write_column<T, ENT, TOP>(q, col, x0, st, list); return; }
+    Stat st = join_lanes<ENT, 32>({a.m, a.s.x + a.s.y, ENT ? a.t.x + a.t.y : 0.f}, c);
+    if (!BLOCK) { write_column<T, ENT, TOP>(q, col, given, given_logit, st, list); return; }
 
-    // the sums of n warps, in warp 0
-    auto join = [&](int n) {
-        if (lane == 0) stats[warp] = st;
-        __syncthreads();
-        if (warp == 0) {
-            st = stats[0];
-            for (int w = 1; w < n; w++) st = merge(st, stats[w], c);
-        }
-    };
-    join(WARPS);
+    if (lane == 0) stats[warp] = st;
+    __syncthreads();
+    if (warp == 0) st = join_lanes<ENT, WARPS>(stats[lane % WARPS], c);
     if (parts > 1) {
         cluster_wait();
         if (warp == 0) {
@@ -454,13 +544,14 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
         cluster_arrive();
         cluster_wait();
         if (part != 0) return;
-        st = part_stats[min(warp, parts - 1)];
-        if (TOP) list = part_lists[min(warp, parts - 1)][lane];
-        __syncthreads();
-        join(parts);
-        if (TOP) list = merge_warps(list, lists, parts);
+        if (warp == 0) st = join_lanes<ENT, 8>(lane % 8 < parts ? part_stats[lane % 8] : Stat{-INFINITY, 0.f, 0.f}, c);
+        if (TOP) {
+            list = part_lists[min(warp, parts - 1)][lane];
+            __syncthreads();                                    // `lists` is read above
+            list = merge_warps(list, lists, parts);
+        }
     }
-    if (warp == 0) write_column<T, ENT, TOP>(q, col, x0, st, list);
+    if (warp == 0) write_column<T, ENT, TOP>(q, col, given, given_logit, st, list);
 }
 
 template <class T, bool ENT, bool TOP>
@@ -469,19 +560,29 @@ static int logprob_go(const LogprobArgs& q, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(256);
     cfg.stream = st;
-    if (nvec <= 512 && q.ncols >= 4 * sm_count()) {
+#ifndef SHORT
+#define SHORT 512
+#endif
+    if (nvec <= SHORT && q.ncols >= 4 * sm_count()) {
         cfg.gridDim = dim3((q.ncols + 7) / 8);
         CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, TOP, 32>, q, 1));
         return CUVDIA_OK;
     }
-    // Waves of blocks (four fit an SM) times what a block takes: its chunks of 1024 vectors and about one chunk's time to
-    // start and to join its warps, two with a list of candidates.
+    // What a call takes, in fifths of the time an SM needs to bring in a chunk of 16 KB: a block's chunks, each at the rate its
+    // SM's blocks leave it but no faster than a round trip to memory allows, and the join of a cluster's blocks (3 us).
     int parts = 1;
     long long best = 0;
     for (int p = 1; p <= 8; p *= 2) {
-        const long long slots = 4 * sm_count(), waves = ((long long)q.ncols * p + slots - 1) / slots;
-        const long long cost = waves * ((nvec + 1024 * p - 1) / (1024 * p) + (TOP ? 2 : 1));
+        const long long chunks = (nvec + 1024 * p - 1) / (1024 * p), per_sm = ((long long)q.ncols * p + sm_count() - 1) / sm_count();
+        const long long cost = chunks * std::max(5 * per_sm, 6LL) + (p > 1 ? 40 : 0);
         if (p == 1 || cost < best) { parts = p; best = cost; }
+    }
+    // Many columns: smaller blocks, of which a thread's share of the joins is smaller.
+    if (parts == 1 && q.ncols >= 4 * sm_count()) {
+        cfg.blockDim = dim3(128);
+        cfg.gridDim = dim3(q.ncols);
+        CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, TOP, 128>, q, 1));
+        return CUVDIA_OK;
     }
     if ((long long)q.ncols * parts > 2147483647LL) { set_last_error("token_logprob: too many columns"); return CUVDIA_ERR_UNSUPPORTED; }
     cfg.gridDim = dim3((unsigned)(q.ncols * parts));
