@@ -45,18 +45,23 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
     return a;
 }
 
-// the largest of a vector's elements, NaN left out
+// the largest and the smallest of a vector's elements, NaN left out
 __device__ __forceinline__ float max_raw(const uint4& r, float) {
     return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
 }
-#define CUVDIA_RAW16(H, H2)                                                                                                    \
-    __device__ __forceinline__ float max_raw(const uint4& r, H) {                                                              \
-        const H2* h = reinterpret_cast<const H2*>(&r);                                                                         \
-        const H2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));                                                        \
-        return fmaxf(to_f32(m.x), to_f32(m.y));                                                                                \
+__device__ __forceinline__ float min_raw(const uint4& r, float) {
+    return fminf(fminf(__uint_as_float(r.x), __uint_as_float(r.y)), fminf(__uint_as_float(r.z), __uint_as_float(r.w)));
+}
+#define CUVDIA_RAW16(H, H2, NAME, PAIRS, SINGLE)                                \
+    __device__ __forceinline__ float NAME(const uint4& r, H) {                  \
+        const H2* h = reinterpret_cast<const H2*>(&r);                          \
+        const H2 m = PAIRS(PAIRS(h[0], h[1]), PAIRS(h[2], h[3]));               \
+        return SINGLE(to_f32(m.x), to_f32(m.y));                                \
     }
-CUVDIA_RAW16(__half, __half2)
-CUVDIA_RAW16(__nv_bfloat16, __nv_bfloat162)
+CUVDIA_RAW16(__half, __half2, max_raw, __hmax2, fmaxf)
+CUVDIA_RAW16(__half, __half2, min_raw, __hmin2, fminf)
+CUVDIA_RAW16(__nv_bfloat16, __nv_bfloat162, max_raw, __hmax2, fmaxf)
+CUVDIA_RAW16(__nv_bfloat16, __nv_bfloat162, min_raw, __hmin2, fminf)
 #undef CUVDIA_RAW16
 
 template <class T> __device__ __forceinline__ unsigned minus_inf_word();
@@ -560,10 +565,7 @@ static int logprob_go(const LogprobArgs& q, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(256);
     cfg.stream = st;
-#ifndef SHORT
-#define SHORT 512
-#endif
-    if (nvec <= SHORT && q.ncols >= 4 * sm_count()) {
+    if (nvec <= 1024 && q.ncols >= 8 * sm_count()) {
         cfg.gridDim = dim3((q.ncols + 7) / 8);
         CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, TOP, 32>, q, 1));
         return CUVDIA_OK;
@@ -614,62 +616,85 @@ int launch_token_logprob(const void* logits, int ld, int type, int vocab, int nc
 
 // ---- gradient ------------------------------------------------------------------------------------------------------
 //   dlogits_v = scale * (dlogp * ([v = token] - p_v) - dentropy * p_v * (log p_v + entropy)),   p_v = exp(scale * logit_v - lse)
-// Element-wise once lse and entropy are known: a block owns up to 1024 vectors of one column.  Vectors are those of the
-// logits' memory; the stores are vectors too where dlogits lies alike (VEC), else element by element.  In place is fine:
-// a thread reads its elements before it writes them.
-template <class T>
+// Element-wise once lse and entropy are known: with d = scale * logit - lse,
+//   dlogits_v = 2^(d log2 e) * (A d + B) (+ scale * dlogp at the token),   A = -scale dentropy,  B = -scale (dlogp + dentropy entropy)
+// two elements an instruction.  A block owns up to 1024 vectors of one column, those of the logits' memory; the stores are vectors
+// too where dlogits lies alike, else element by element.  In place is fine: a thread reads its elements before it writes them.
+struct GradFactors { float scale, minus_lse, a, b; };
+
+// a vector's gradients but for the token's own term; CUT: exponents are cut, see LEAST
+template <class T, bool ENT, bool CUT>
+__device__ __forceinline__ void grad_vector(float (&x)[Vec16<T>::N], const GradFactors& f) {
+#pragma unroll
+    for (int e = 0; e < Vec16<T>::N; e += 2) {
+        float2 d = __ffma2_rn(make_float2(x[e], x[e + 1]), make_float2(f.scale, f.scale), make_float2(f.minus_lse, f.minus_lse));
+        const float2 q = __fmul2_rn(d, make_float2(LOG2E, LOG2E));
+        const float2 p = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+        if (ENT && CUT) d = make_float2(fmaxf(d.x, LEAST), fmaxf(d.y, LEAST));
+        const float2 b = make_float2(f.b, f.b);
+        const float2 r = __fmul2_rn(p, ENT ? __ffma2_rn(d, make_float2(f.a, f.a), b) : b);
+        x[e] = r.x; x[e + 1] = r.y;
+    }
+}
+
+template <class T, bool ENT>
 __global__ void __launch_bounds__(256)
-token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long ld, int vocab, int ncols,
-                          const Tokens tokens, float scale, const float* __restrict__ lse,
-                          const float* __restrict__ dlogp, const float* __restrict__ entropy,
+token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long ld, int vocab, const Tokens tokens, float scale,
+                          const float* __restrict__ lse, const float* __restrict__ dlogp, const float* __restrict__ entropy,
                           const float* __restrict__ dentropy, int chunks) {
-    constexpr int V = Vec16<T>::N, U = 4;
+    constexpr int V = Vec16<T>::N;
+    const int threads = blockDim.x;
     const long long col = blockIdx.x / (unsigned)chunks;
     const int chunk = blockIdx.x - (unsigned)col * (unsigned)chunks;
     const T* x0 = logits + col * ld;
     T* y0 = dlogits + col * ldd;
-    const int head = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
+    const int head = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));      // elements before x0 in its first vector
     const bool alike = ((reinterpret_cast<uintptr_t>(x0) ^ reinterpret_cast<uintptr_t>(y0)) & 15) == 0;
+    const float l = lse[col];
     long long t = dlogp ? tokens[col] : -1;
     if (t < 0 || t >= vocab) t = -1;
-    const float g = t >= 0 ? dlogp[col] : 0.f, h = dentropy ? dentropy[col] : 0.f, l = lse[col];
-    const float ent = dentropy ? entropy[col] : 0.f;
     // A padded column without an entropy term is zero without a look at its logits, and so is a column that has no
     // finite logit.
-    const bool zero = (t < 0 && dentropy == nullptr) || l == -INFINITY;
-    const int i0 = chunk * 256 * U + threadIdx.x;
-    float x[U][V];
+    const bool zero = (t < 0 && !ENT) || l == -INFINITY;
+    const int first = (chunk * (threads * U) + (int)threadIdx.x) * V - head;
+    uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const long long e0 = ((long long)i0 + u * 256) * V - head;
+        const int e0 = first + u * (threads * V);
+        if (!zero && e0 >= 0 && e0 + V <= vocab) raw[u] = *reinterpret_cast<const uint4*>(x0 + e0);
+    }
+    const float g = t >= 0 ? dlogp[col] : 0.f, h = ENT ? dentropy[col] : 0.f, hot = scale * g;
+    const GradFactors f = {scale, -l, -scale * h, -scale * (ENT ? fmaf(h, entropy[col], g) : g)};
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int e0 = first + u * (threads * V);
+        if (e0 >= vocab) break;
+        const bool whole = e0 >= 0 && e0 + V <= vocab;
+        float x[V];
         if (zero) {
 #pragma unroll
-            for (int e = 0; e < V; e++) x[u][e] = 0.f;
-        } else if (e0 >= 0 && e0 + V <= vocab) {
-            unpack16<T>(*reinterpret_cast<const uint4*>(x0 + e0), x[u]);
+            for (int e = 0; e < V; e++) x[e] = 0.f;
         } else {
+            if (whole) {
+                unpack16<T>(raw[u], x);
+            } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) x[u][e] = e0 + e >= 0 && e0 + e < vocab ? to_f32(x0[e0 + e]) : 0.f;
-        }
-    }
+                for (int e = 0; e < V; e++) x[e] = e0 + e >= 0 && e0 + e < vocab ? to_f32(x0[e0 + e]) : 0.f;
+            }
+            // 0 * -inf comes up only where the least exponent is out of all proportion (a forbidden token)
+            if (ENT && (!whole || fmaf(min_raw(raw[u], T()), scale, -l) < LEAST)) grad_vector<T, ENT, true>(x, f);
+            else grad_vector<T, ENT, false>(x, f);
+            const unsigned at = (unsigned)((int)t - e0);
+            if (at < V && t >= 0) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const long long e0 = ((long long)i0 + u * 256) * V - head;
-        if (e0 >= vocab) break;
-        if (!zero) {
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float d = fmaf(x[u][e], scale, -l), p = exp2_approx(d * LOG2E);
-                const float w = dentropy ? fmaf(h, fmaxf(d, LEAST) + ent, g) : g;
-                const float hot = e0 + e == t ? g : 0.f;
-                x[u][e] = scale * fmaf(-p, w, hot);
+                for (int e = 0; e < V; e++) if (e == (int)at) x[e] += hot;
             }
         }
-        if (alike && e0 >= 0 && e0 + V <= vocab) {
-            *reinterpret_cast<uint4*>(y0 + e0) = pack16<T>(x[u]);
+        if (alike && whole) {
+            *reinterpret_cast<uint4*>(y0 + e0) = pack16<T>(x);
         } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) if (e0 + e >= 0 && e0 + e < vocab) y0[e0 + e] = from_f32<T>(x[u][e]);
+            for (int e = 0; e < V; e++) if (e0 + e >= 0 && e0 + e < vocab) y0[e0 + e] = from_f32<T>(x[e]);
         }
     }
 }
@@ -678,11 +703,15 @@ int launch_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld
                               const void* tokens, int token_type, float scale, const float* lse, const float* dlogp,
                               const float* entropy, const float* dentropy, cudaStream_t st) {
     const int v = 16 / type_size(type);
-    const long long chunks = ((long long)vocab + v - 1 + 1024 * v - 1) / (1024 * v);       // up to v - 1 elements of offset
+    // blocks of 1024 vectors, of fewer where a column has no more
+    const int threads = vocab > 512 * v ? 256 : vocab > 256 * v ? 128 : 64;
+    const long long per = threads * U * v, chunks = ((long long)vocab + v - 1 + per - 1) / per;       // up to v - 1 elements of offset
     const long long blocks = chunks * ncols;
     if (blocks > 2147483647LL) { set_last_error("token_logprob_grad: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
-    CUVDIA_FLOAT_TYPE(type, (token_logprob_grad_kernel<T><<<(unsigned)blocks, 256, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld,
-        vocab, ncols, make_tokens(tokens, token_type), scale, lse, dlogp, entropy, dentropy, (int)chunks)));
+#define LG_GO(E) token_logprob_grad_kernel<T, E><<<(unsigned)blocks, threads, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld, vocab, \
+    make_tokens(tokens, token_type), scale, lse, dlogp, entropy, dentropy, (int)chunks)
+    CUVDIA_FLOAT_TYPE(type, { if (dentropy) LG_GO(true); else LG_GO(false); });
+#undef LG_GO
     count_launch();
     return check_launch("token_logprob_grad_kernel");
 }
