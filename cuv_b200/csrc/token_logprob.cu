@@ -637,13 +637,12 @@ __device__ __forceinline__ void grad_vector(float (&x)[Vec16<T>::N], const GradF
     }
 }
 
-template <class T, bool ENT>
-__global__ void __launch_bounds__(256)
+template <class T, bool ENT, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long ld, int vocab, const Tokens tokens, float scale,
                           const float* __restrict__ lse, const float* __restrict__ dlogp, const float* __restrict__ entropy,
                           const float* __restrict__ dentropy, int chunks) {
     constexpr int V = Vec16<T>::N;
-    const int threads = blockDim.x;
     const long long col = blockIdx.x / (unsigned)chunks;
     const int chunk = blockIdx.x - (unsigned)col * (unsigned)chunks;
     const T* x0 = logits + col * ld;
@@ -656,18 +655,18 @@ token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long 
     // A padded column without an entropy term is zero without a look at its logits, and so is a column that has no
     // finite logit.
     const bool zero = (t < 0 && !ENT) || l == -INFINITY;
-    const int first = (chunk * (threads * U) + (int)threadIdx.x) * V - head;
+    const int first = (chunk * (THREADS * U) + (int)threadIdx.x) * V - head;
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int e0 = first + u * (threads * V);
+        const int e0 = first + u * (THREADS * V);
         if (!zero && e0 >= 0 && e0 + V <= vocab) raw[u] = *reinterpret_cast<const uint4*>(x0 + e0);
     }
     const float g = t >= 0 ? dlogp[col] : 0.f, h = ENT ? dentropy[col] : 0.f, hot = scale * g;
     const GradFactors f = {scale, -l, -scale * h, -scale * (ENT ? fmaf(h, entropy[col], g) : g)};
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int e0 = first + u * (threads * V);
+        const int e0 = first + u * (THREADS * V);
         if (e0 >= vocab) break;
         const bool whole = e0 >= 0 && e0 + V <= vocab;
         float x[V];
@@ -704,13 +703,16 @@ int launch_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld
                               const float* entropy, const float* dentropy, cudaStream_t st) {
     const int v = 16 / type_size(type);
     // blocks of 1024 vectors, of fewer where a column has no more
-    const int threads = vocab > 512 * v ? 256 : vocab > 256 * v ? 128 : 64;
+    const int threads = vocab > 256 * v ? 256 : 64;
     const long long per = threads * U * v, chunks = ((long long)vocab + v - 1 + per - 1) / per;       // up to v - 1 elements of offset
     const long long blocks = chunks * ncols;
     if (blocks > 2147483647LL) { set_last_error("token_logprob_grad: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
-#define LG_GO(E) token_logprob_grad_kernel<T, E><<<(unsigned)blocks, threads, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld, vocab, \
-    make_tokens(tokens, token_type), scale, lse, dlogp, entropy, dentropy, (int)chunks)
-    CUVDIA_FLOAT_TYPE(type, { if (dentropy) LG_GO(true); else LG_GO(false); });
+#define LG_GO(E, N) token_logprob_grad_kernel<T, E, N><<<(unsigned)blocks, N, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld, \
+    vocab, make_tokens(tokens, token_type), scale, lse, dlogp, entropy, dentropy, (int)chunks)
+    CUVDIA_FLOAT_TYPE(type, {
+        if (threads == 256) { if (dentropy) LG_GO(true, 256); else LG_GO(false, 256); }
+        else                { if (dentropy) LG_GO(true, 64); else LG_GO(false, 64); }
+    });
 #undef LG_GO
     count_launch();
     return check_launch("token_logprob_grad_kernel");
