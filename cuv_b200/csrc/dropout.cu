@@ -19,95 +19,189 @@ struct DropoutArgs {
     float scale;
 };
 
-__device__ __forceinline__ uint4 draw_words(const DropoutArgs& a, unsigned group, long long gcol) {
-    uint4 c = make_uint4(group, (unsigned)gcol, a.which + 65536u * (unsigned)(gcol >> 32), a.step);
+constexpr unsigned M0 = 0xD2511F53u, M1 = 0xCD9E8D57u;
+
+// The four words of a group of rows; first = M0 * group, the first round's product, which a caller that walks through a column
+// adds up instead of multiplying.
+__device__ __forceinline__ uint4 draw_words(const DropoutArgs& a, unsigned long long first, long long gcol) {
+    const unsigned long long second = (unsigned long long)M1 * (a.which + 65536u * (unsigned)(gcol >> 32));
+    uint4 c = make_uint4((unsigned)(second >> 32) ^ (unsigned)gcol ^ a.key0[0], (unsigned)second,
+                         (unsigned)(first >> 32) ^ a.step ^ a.key1[0], (unsigned)first);
 #pragma unroll
-    for (int r = 0; r < 10; r++) {
-        const unsigned long long p0 = (unsigned long long)0xD2511F53u * c.x, p1 = (unsigned long long)0xCD9E8D57u * c.z;
+    for (int r = 1; r < 10; r++) {
+        const unsigned long long p0 = (unsigned long long)M0 * c.x, p1 = (unsigned long long)M1 * c.z;
         c = make_uint4((unsigned)(p1 >> 32) ^ c.y ^ a.key0[r], (unsigned)p1, (unsigned)(p0 >> 32) ^ c.w ^ a.key1[r], (unsigned)p0);
     }
     return c;
 }
 
-// A thread owns U runs of N = 8 consecutive rows of one column, `lanes` runs apart (`lanes` threads, a power of two, work on one
-// column of the block, 256 / lanes columns on one block); all of its loads are in flight before the first number is drawn.
-// NONE: p = 1, every element is dropped.
-template <class T, bool RESIDUAL, bool ALIGNED, bool NONE>
-__global__ void __launch_bounds__(256)
-dropout_kernel(T* dst, long long ldd, const T* src, long long lds, const T* residual, long long ldr, int rows, int ncols,
-               int lanes, int chunks, const DropoutArgs a) {
-    constexpr int N = 8, U = 2, W = N / Vec16<T>::N;
-    const unsigned group = blockIdx.x / (unsigned)chunks, chunk = blockIdx.x - group * (unsigned)chunks;
-    const int sub = threadIdx.x / lanes, lane = threadIdx.x - sub * lanes;
-    const long long col = (long long)group * (256 / lanes) + sub;
-    if (col >= ncols) return;
-    const long long gcol = a.col0 + col;
-    const T* s = src + col * lds;
-    const T* r = RESIDUAL ? residual + col * ldr : nullptr;
-    T* d = dst + col * ldd;
-    const int i0 = ((int)chunk * U * lanes + lane) * N;
-    uint4 xs[U][W], rs[U][W];
+// One word per element for the rows from a group of four on
+template <int WORDS>
+__device__ __forceinline__ void draw(const DropoutArgs& a, unsigned long long first, long long gcol, unsigned (&word)[WORDS]) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int i = i0 + u * lanes * N;
-        if (ALIGNED && i + N <= rows) {
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                xs[u][w] = reinterpret_cast<const uint4*>(s + i)[w];
-                if (RESIDUAL) rs[u][w] = reinterpret_cast<const uint4*>(r + i)[w];
-            }
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int i = i0 + u * lanes * N;
-        if (i >= rows) break;
-        const bool whole = ALIGNED && i + N <= rows;
-        float x[N], y[N];
-        if (whole) {
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                float v[Vec16<T>::N];
-                unpack16<T>(xs[u][w], v);
-#pragma unroll
-                for (int e = 0; e < Vec16<T>::N; e++) x[w * Vec16<T>::N + e] = v[e];
-                if (RESIDUAL) {
-                    unpack16<T>(rs[u][w], v);
-#pragma unroll
-                    for (int e = 0; e < Vec16<T>::N; e++) y[w * Vec16<T>::N + e] = v[e];
-                }
-            }
-        } else {
-            load_run<T, N, false>(s + i, rows - i, x);
-            if (RESIDUAL) load_run<T, N, false>(r + i, rows - i, y);
-        }
-#pragma unroll
-        for (int q = 0; q < N / 4; q++) {
-            const uint4 w = draw_words(a, (unsigned)(i >> 2) + q, gcol);
-            const unsigned word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float kept = !NONE && word[e] >= a.least ? x[4 * q + e] * a.scale : 0.f;
-                x[4 * q + e] = RESIDUAL ? kept + y[4 * q + e] : kept;
-            }
-        }
-        if (whole) store_run<T, N, true>(d + i, N, x);
-        else store_run<T, N, false>(d + i, rows - i, x);
+    for (int q = 0; q < WORDS / 4; q++) {
+        const uint4 w = draw_words(a, first + (unsigned long long)M0 * q, gcol);
+        word[4 * q] = w.x; word[4 * q + 1] = w.y; word[4 * q + 2] = w.z; word[4 * q + 3] = w.w;
     }
 }
 
-template <class T, bool RESIDUAL, bool ALIGNED>
-static int dropout_go(void* dst, int ldd, const void* src, int lds, const void* residual, int ldr, int rows, int ncols, bool none,
-                      const DropoutArgs& a, cudaStream_t st) {
-    constexpr int N = 8, U = 2;
-    const long long items = ((long long)rows + U * N - 1) / (U * N);
-    int lanes = 1;
-    while (lanes < 256 && lanes < items) lanes *= 2;
-    const long long chunks = (items + lanes - 1) / lanes, per = 256 / lanes, blocks = (ncols + per - 1) / per * chunks;
-    if (blocks > 2147483647LL) { set_last_error("dropout: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
-#define DROP_GO(Z) dropout_kernel<T, RESIDUAL, ALIGNED, Z><<<(unsigned)blocks, 256, 0, st>>>((T*)dst, ldd, (const T*)src, lds, \
-    (const T*)residual, ldr, rows, ncols, lanes, (int)chunks, a)
-    if (none) DROP_GO(true); else DROP_GO(false);
+template <class T> struct Streams { T* dst; const T* src; const T* residual; long long ldd, lds, ldr; };
+
+// ---- matrices whose columns lie alike --------------------------------------------------------------------------------
+// A column is walked as the 16-byte vectors of the memory it lies in, E elements each.  Where every column starts on such a
+// vector (SHIFTED = false) a vector's rows are whole groups of the generator.  Where columns start h elements into one (the
+// same h in all matrices), the rows of vector k are E*k - h ..: a lane draws for the rows E*k .. and takes the other h
+// decisions from the lane before it, so nothing is drawn twice but one lane's share of a part.
+// `lanes` threads (a power of two; of one warp if SHIFTED) take a part of a column, U vectors each, `lanes` vectors apart: all loads are in
+// flight before the first number is drawn.  The generator's 32 x 32 bit products keep the heavy multiplier pipe
+// 70 % busy in 16-bit types, where it takes as long as the memory traffic.
+// WIDE: a part is a block's.  NONE: p = 1, every element is dropped.
+template <class T, bool RESIDUAL, bool SHIFTED, bool NONE, int U, bool WIDE>
+__global__ void __launch_bounds__(256, SHIFTED || RESIDUAL ? 4 : 5)
+dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts, const DropoutArgs a) {
+    constexpr int E = Vec16<T>::N;
+    const int lanes = WIDE ? 256 : 1 << log_lanes, l = threadIdx.x & (lanes - 1), span = lanes * U - (SHIFTED ? 1 : 0);
+    long long col;
+    int part;
+    if (WIDE) {                                                 // one part a block
+        col = (long long)blockIdx.z * gridDim.y + blockIdx.y;
+        part = blockIdx.x;
+    } else {
+        const unsigned team = blockIdx.x * (256u >> log_lanes) + (threadIdx.x >> log_lanes);
+        col = team / (unsigned)parts;
+        part = (int)(team - (unsigned)col * (unsigned)parts);
+    }
+    const bool idle = col >= ncols;
+    if (!SHIFTED && idle) return;
+    if (idle) col = 0;
+    const T* s = m.src + col * m.lds;
+    const T* r = RESIDUAL ? m.residual + col * m.ldr : nullptr;
+    T* d = m.dst + col * m.ldd;
+    const int h = SHIFTED ? (int)((reinterpret_cast<uintptr_t>(d) & 15) / sizeof(T)) : 0;
+    const int w0 = part * span + l, i0 = w0 * E - h;
+    uint4 xs[U], rs[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = i0 + u * lanes * E;
+        if (!idle && (!SHIFTED || i >= 0) && i + E <= rows) {
+            xs[u] = *reinterpret_cast<const uint4*>(s + i);
+            if (RESIDUAL) rs[u] = *reinterpret_cast<const uint4*>(r + i);
+        }
+    }
+    const long long gcol = a.col0 + col;
+    unsigned long long first = (unsigned long long)M0 * (unsigned)(w0 * (E / 4));
+    const unsigned long long first_step = (unsigned long long)M0 * (unsigned)(lanes * (E / 4));
+    unsigned before = 0;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = i0 + u * lanes * E;
+        if (!SHIFTED && i >= rows) break;
+        unsigned word[E], mask = 0;
+        if (!NONE) draw<E>(a, first, gcol, word);
+        first += first_step;
+        if (SHIFTED) {
+            if (!NONE) {
+#pragma unroll
+                for (int e = 0; e < E; e++) mask |= word[e] >= a.least ? 1u << e : 0u;
+            }
+            unsigned prev = __shfl_up_sync(0xffffffffu, mask, 1, lanes);
+            const unsigned last = __shfl_sync(0xffffffffu, before, lanes - 1, lanes);
+            if (u > 0 && l == 0) prev = last;
+            before = mask;
+            mask = (prev | mask << E) >> (E - h);
+            if (idle || i >= rows || (part > 0 && u == 0 && l == 0)) continue;         // that lane only drew for the next one
+        }
+        const bool whole = (!SHIFTED || i >= 0) && i + E <= rows;
+        float x[E], y[E];
+        if (whole) {
+            unpack16<T>(xs[u], x);
+            if (RESIDUAL) unpack16<T>(rs[u], y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const bool in = i + e >= 0 && i + e < rows;
+                x[e] = in ? to_f32(s[i + e]) : 0.f;
+                if (RESIDUAL) y[e] = in ? to_f32(r[i + e]) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float2 scaled = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(a.scale, a.scale));
+            const bool keep0 = SHIFTED ? mask >> e & 1 : !NONE && word[e] >= a.least;
+            const bool keep1 = SHIFTED ? mask >> (e + 1) & 1 : !NONE && word[e + 1] >= a.least;
+            const float2 kept = make_float2(keep0 ? scaled.x : 0.f, keep1 ? scaled.y : 0.f);
+            const float2 sum = RESIDUAL ? __fadd2_rn(kept, make_float2(y[e], y[e + 1])) : kept;
+            x[e] = sum.x; x[e + 1] = sum.y;
+        }
+        if (whole) {
+            *reinterpret_cast<uint4*>(d + i) = pack16<T>(x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) if (i + e >= 0 && i + e < rows) d[i + e] = from_f32<T>(x[e]);
+        }
+    }
+}
+
+// ---- any layout --------------------------------------------------------------------------------------------------------
+// Matrices that lie differently: four rows, one group of the generator, a thread, element by element.
+template <class T, bool RESIDUAL>
+__global__ void __launch_bounds__(256)
+dropout_any_kernel(const Streams<T> m, int rows, int ncols, long long groups, bool none, const DropoutArgs a) {
+    const long long t = (long long)blockIdx.x * 256 + threadIdx.x, col = t / groups;
+    if (col >= ncols) return;
+    const int i = (int)(t - col * groups) * 4;
+    unsigned word[4];
+    draw<4>(a, (unsigned long long)M0 * (unsigned)(i >> 2), a.col0 + col, word);
+    const T* src = m.src + col * m.lds + i;
+    const T* residual = RESIDUAL ? m.residual + col * m.ldr + i : nullptr;
+    float x[4], r[4];
+    load_run<T, 4, false>(src, rows - i, x);
+    if (RESIDUAL) load_run<T, 4, false>(residual, rows - i, r);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float kept = !none && word[e] >= a.least ? x[e] * a.scale : 0.f;
+        x[e] = RESIDUAL ? kept + r[e] : kept;
+    }
+    store_run<T, 4, false>(m.dst + col * m.ldd + i, rows - i, x);
+}
+
+template <class T, bool RESIDUAL>
+static int dropout_go(const Streams<T>& m, int rows, int ncols, bool none, const DropoutArgs& a, cudaStream_t st) {
+    const auto alike = [&](const T* p, long long ld) {
+        return ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(m.dst)) & 15) == 0 && ((ld - m.ldd) * (long long)sizeof(T)) % 16 == 0;
+    };
+    if (!alike(m.src, m.lds) || (RESIDUAL && !alike(m.residual, m.ldr))) {
+        const long long groups = (rows + 3) / 4, blocks = (groups * ncols + 255) / 256;
+        if (blocks > 2147483647LL) { set_last_error("dropout: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
+        dropout_any_kernel<T, RESIDUAL><<<(unsigned)blocks, 256, 0, st>>>(m, rows, ncols, groups, none, a);
+        count_launch();
+        return check_launch("dropout_any_kernel");
+    }
+    constexpr int E = Vec16<T>::N;
+    const bool shifted = !columns16(m.dst, m.ldd, sizeof(T));
+    const long long vectors = ((long long)rows + E - 1 + (shifted ? E - 1 : 0)) / E, per = shifted ? 3 : 4;
+    // As many lanes a part as leave at most an eighth of a column's parts empty, a whole block at best: its vectors lie
+    // together and its column is known without a division (16384 x 8192 bf16 with residual: 138 us, by warps 150 us).
+    int log_lanes = 0;
+    while (log_lanes < 5 && (per << log_lanes) < vectors) log_lanes++;
+    if (!shifted)
+        for (int k = 6; k <= 8; k++) {
+            const long long block = per << k;
+            if ((vectors + block - 1) / block * block - vectors <= vectors / 8) log_lanes = k;
+        }
+    const long long span = (per << log_lanes) - (shifted ? 1 : 0);
+    const long long parts = vectors <= per << log_lanes ? 1 : (vectors + span - 1) / span, teams = parts * ncols;
+    const long long y = std::min((long long)ncols, 32768LL);
+    const long long blocks = log_lanes == 8 ? parts : (teams + (256 >> log_lanes) - 1) >> (8 - log_lanes);
+    if (teams > 4294967295LL || blocks > 2147483647LL) { set_last_error("dropout: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
+    const dim3 grid((unsigned)blocks, log_lanes == 8 ? (unsigned)y : 1, log_lanes == 8 ? (unsigned)((ncols + y - 1) / y) : 1);
+#define DROP_GO(SH, U, W) do {                                                                                                     \
+        if (none) dropout_kernel<T, RESIDUAL, SH, true, U, W><<<grid, 256, 0, st>>>(m, rows, ncols, log_lanes, (int)parts, a);      \
+        else dropout_kernel<T, RESIDUAL, SH, false, U, W><<<grid, 256, 0, st>>>(m, rows, ncols, log_lanes, (int)parts, a);          \
+    } while (0)
+    if (shifted) DROP_GO(true, 3, false);
+    else if (log_lanes == 8) DROP_GO(false, 4, true);
+    else DROP_GO(false, 4, false);
 #undef DROP_GO
     count_launch();
     return check_launch("dropout_kernel");
@@ -115,8 +209,6 @@ static int dropout_go(void* dst, int ldd, const void* src, int lds, const void* 
 
 int launch_dropout(void* dst, int ldd, const void* src, int lds, const void* residual, int ldr, int type, int rows,
                    int ncols, float p, const DrawParams& d, cudaStream_t st) {
-    const int size = type_size(type);
-    const bool aligned = columns16(dst, ldd, size) && columns16(src, lds, size) && (!residual || columns16(residual, ldr, size));
     DropoutArgs a;
     for (int r = 0; r < 10; r++) { a.key0[r] = d.k0 + r * 0x9E3779B9u; a.key1[r] = d.k1 + r * 0xBB67AE85u; }
     a.which = d.which; a.step = d.step; a.col0 = d.col0;
@@ -125,10 +217,8 @@ int launch_dropout(void* dst, int ldd, const void* src, int lds, const void* res
     a.scale = none ? 0.f : (float)(1.0 / (1.0 - (double)p));
     int rc = CUVDIA_OK;
     CUVDIA_FLOAT_TYPE(type, {
-        if (residual) rc = aligned ? dropout_go<T, true, true>(dst, ldd, src, lds, residual, ldr, rows, ncols, none, a, st)
-                                   : dropout_go<T, true, false>(dst, ldd, src, lds, residual, ldr, rows, ncols, none, a, st);
-        else rc = aligned ? dropout_go<T, false, true>(dst, ldd, src, lds, residual, ldr, rows, ncols, none, a, st)
-                          : dropout_go<T, false, false>(dst, ldd, src, lds, residual, ldr, rows, ncols, none, a, st);
+        const Streams<T> m = {(T*)dst, (const T*)src, (const T*)residual, ldd, lds, ldr};
+        rc = residual ? dropout_go<T, true>(m, rows, ncols, none, a, st) : dropout_go<T, false>(m, rows, ncols, none, a, st);
     });
     return rc;
 }

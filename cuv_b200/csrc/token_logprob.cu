@@ -282,13 +282,6 @@ __device__ __forceinline__ Stat join_lanes(Stat r, float c) {
 // The vectors of a column on their way through shared memory: a thread copies its own vectors in asynchronously, some chunks
 // ahead, and reads back what it copied itself, so that no barrier is involved and vectors in flight hold no registers.
 
-__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-
 template <class T>
 __device__ __forceinline__ float max_chunk(const uint4* v, int step) {
     float m = max_raw(v[0], T());
@@ -448,11 +441,11 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
         uint4* slot = mine + to * (U * THREADS);
         if (ahead + STEP * U <= v1) {
 #pragma unroll
-            for (int u = 0; u < U; u++) copy_async(slot + u * THREADS, from + u * STEP);
+            for (int u = 0; u < U; u++) copy_async16(slot + u * THREADS, from + u * STEP);
         } else if (ahead < v1) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                if (ahead + u * STEP + tid < v1) copy_async(slot + u * THREADS, from + u * STEP);
+                if (ahead + u * STEP + tid < v1) copy_async16(slot + u * THREADS, from + u * STEP);
                 else slot[u * THREADS] = make_uint4(nothing, nothing, nothing, nothing);
             }
         }

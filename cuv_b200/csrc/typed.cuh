@@ -63,6 +63,15 @@ __device__ __forceinline__ uint4 pack16(const float (&x)[Vec16<T>::N]) {
     }
 }
 
+// 16 bytes into shared memory without a register on the way (both addresses 16-byte aligned).  A thread may read what it
+// copied itself once copies_wait<n> has returned: all of its groups of copies but the n youngest are complete then.
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
 // N consecutive elements at p: one 128-bit access per 16 bytes (p 16-byte aligned), or, where ALIGNED is false or the
 // range ends inside, element by element up to `n` of them.
 template <class T, int N, bool ALIGNED>
