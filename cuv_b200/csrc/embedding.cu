@@ -6,61 +6,103 @@
 
 namespace cuvdia {
 
-static inline int lanes_for(long long items) {
-    int lanes = 1;
-    while (lanes < 256 && lanes < items) lanes *= 2;
-    return lanes;
-}
-
 // ---- lookup -----------------------------------------------------------------------------------------------------
-// `lanes` threads (a power of two) share a column, 256 / lanes columns a block; a thread moves up to four runs of N
-// elements of its column, all loads before the first store.
-template <class T, int N, bool ALIGNED>
+// `lanes` threads (a power of two) take a part of a column of dst, U of the 16-byte vectors of the memory it lies in each, `lanes`
+// vectors apart, and keep them as they are until they are stored: all loads are in flight before the first store.  Where columns
+// do not start on such vectors (ALIGNED = false) a vector's elements straddle two vectors of the table, which are loaded both
+// and shifted into place, so that only the ends of a column are moved element by element.
+template <class T, bool ALIGNED, bool WIDE>
 __global__ void __launch_bounds__(256)
 embedding_kernel(T* __restrict__ dst, long long ldd, const T* __restrict__ table, long long ldt, int units, int vocab,
-                 const Tokens tokens, int ncols, float scale, int lanes, int chunks) {
-    constexpr int U = 4;
-    const unsigned group = blockIdx.x / (unsigned)chunks, chunk = blockIdx.x - group * (unsigned)chunks;
-    const int sub = threadIdx.x / lanes, lane = threadIdx.x - sub * lanes;
-    const long long col = (long long)group * (256 / lanes) + sub;
+                 const Tokens tokens, int ncols, float scale, int log_lanes, int parts) {
+    constexpr int U = ALIGNED ? 4 : 2, E = Vec16<T>::N;
+    const int lanes = WIDE ? 256 : 1 << log_lanes, l = threadIdx.x & (lanes - 1);
+    long long col;
+    int part;
+    if (WIDE) {                                                 // one part a block
+        col = (long long)blockIdx.z * gridDim.y + blockIdx.y;
+        part = blockIdx.x;
+    } else {
+        const unsigned team = blockIdx.x * (256u >> log_lanes) + (threadIdx.x >> log_lanes);
+        col = team / (unsigned)parts;
+        part = (int)(team - (unsigned)col * (unsigned)parts);
+    }
     if (col >= ncols) return;
     const long long tok = tokens[col];
     const bool there = tok >= 0 && tok < vocab;
     const T* from = table + (there ? tok : 0) * ldt;
     T* to = dst + col * ldd;
-    float x[U][N];
+    const int i0 = (part * lanes * U + l) * E - (ALIGNED ? 0 : behind16(to));
+    const int r = ALIGNED ? 0 : behind16(from + i0);            // the same for all of a column's vectors
+    uint4 raw[U], more[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const long long i = (((long long)chunk * U + u) * lanes + lane) * N;
-        const int n = there ? (int)max(0LL, min((long long)N, units - i)) : 0;
-        load_run<T, N, ALIGNED>(from + i, n, x[u]);
+        const int i = i0 + u * lanes * E;
+        raw[u] = more[u] = make_uint4(0, 0, 0, 0);
+        if (there && i - r >= 0 && i - r + (r ? 2 : 1) * E <= units) {
+            raw[u] = __ldg(reinterpret_cast<const uint4*>(from + i - r));
+            if (!ALIGNED && r) more[u] = __ldg(reinterpret_cast<const uint4*>(from + i - r) + 1);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const long long i = (((long long)chunk * U + u) * lanes + lane) * N;
+        const int i = i0 + u * lanes * E;
         if (i >= units) break;
+        if (i >= 0 && i + E <= units && (!there || (i - r >= 0 && i - r + (r ? 2 : 1) * E <= units))) {
+            if (!ALIGNED) raw[u] = shift16(raw[u], more[u], r * (int)sizeof(T));
+            if (scale != 1.f && there) {
+                float x[E];
+                unpack16<T>(raw[u], x);
 #pragma unroll
-        for (int e = 0; e < N; e++) x[u][e] = there ? x[u][e] * scale : 0.f;
-        store_run<T, N, ALIGNED>(to + i, (int)min((long long)N, units - i), x[u]);
+                for (int e = 0; e < E; e += 2) {
+                    const float2 y = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(scale, scale));
+                    x[e] = y.x; x[e + 1] = y.y;
+                }
+                raw[u] = pack16<T>(x);
+            }
+            *reinterpret_cast<uint4*>(to + i) = raw[u];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (i + e >= 0 && i + e < units) to[i + e] = from_f32<T>(there ? to_f32(from[i + e]) * scale : 0.f);
+        }
     }
+}
+
+template <class T, bool ALIGNED>
+static int embedding_go(T* dst, int ldd, const T* table, int ldt, int units, int vocab, const Tokens& tokens, int ncols,
+                        float scale, cudaStream_t st) {
+    constexpr long long U = ALIGNED ? 4 : 2;
+    const long long e = Vec16<T>::N, runs = ((long long)units + e - 1 + (ALIGNED ? 0 : e - 1)) / e;
+    // as in dropout.cu: as many lanes a part as leave at most an eighth of a column's parts empty
+    int log_lanes = 0;
+    while (log_lanes < 5 && (U << log_lanes) < runs) log_lanes++;
+    for (int k = 6; k <= 8; k++) {
+        const long long block = U << k;
+        if ((runs + block - 1) / block * block - runs <= runs / 8) log_lanes = k;
+    }
+    const long long span = U << log_lanes, parts = (runs + span - 1) / span, teams = parts * ncols;
+    const long long y = std::min((long long)ncols, 32768LL);
+    const long long blocks = log_lanes == 8 ? parts : (teams + (256 >> log_lanes) - 1) >> (8 - log_lanes);
+    if (teams > 4294967295LL || blocks > 2147483647LL) { set_last_error("embedding: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
+    const dim3 grid((unsigned)blocks, log_lanes == 8 ? (unsigned)y : 1, log_lanes == 8 ? (unsigned)((ncols + y - 1) / y) : 1);
+    if (log_lanes == 8) embedding_kernel<T, ALIGNED, true><<<grid, 256, 0, st>>>(dst, ldd, table, ldt, units, vocab, tokens, ncols, scale, log_lanes, (int)parts);
+    else embedding_kernel<T, ALIGNED, false><<<grid, 256, 0, st>>>(dst, ldd, table, ldt, units, vocab, tokens, ncols, scale, log_lanes, (int)parts);
+    count_launch();
+    return check_launch("embedding_kernel");
 }
 
 int launch_embedding(void* dst, int ldd, const void* table, int ldt, int type, int units, int vocab, const void* tokens,
                      int token_type, int ncols, float scale, cudaStream_t st) {
     const int size = type_size(type);
     const bool aligned = columns16(dst, ldd, size) && columns16(table, ldt, size);
-    const int n = aligned ? 16 / size : 1;
-    const long long items = ((long long)units + 4 * n - 1) / (4 * n);
-    const int lanes = lanes_for(items);
-    const long long chunks = (items + lanes - 1) / lanes, per = 256 / lanes;
-    const long long blocks = (ncols + per - 1) / per * chunks;
-    if (blocks > 2147483647LL) { set_last_error("embedding: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
-#define EMB_GO(N, A) embedding_kernel<T, N, A><<<(unsigned)blocks, 256, 0, st>>>((T*)dst, ldd, (const T*)table, ldt, units, \
-    vocab, make_tokens(tokens, token_type), ncols, scale, lanes, (int)chunks)
-    CUVDIA_FLOAT_TYPE(type, { if (aligned) EMB_GO(Vec16<T>::N, true); else EMB_GO(1, false); });
-#undef EMB_GO
-    count_launch();
-    return check_launch("embedding_kernel");
+    const Tokens toks = make_tokens(tokens, token_type);
+    int rc = CUVDIA_OK;
+    CUVDIA_FLOAT_TYPE(type, {
+        rc = aligned ? embedding_go<T, true>((T*)dst, ldd, (const T*)table, ldt, units, vocab, toks, ncols, scale, st)
+                     : embedding_go<T, false>((T*)dst, ldd, (const T*)table, ldt, units, vocab, toks, ncols, scale, st);
+    });
+    return rc;
 }
 
 // ---- positions sorted by token -----------------------------------------------------------------------------------

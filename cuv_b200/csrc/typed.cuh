@@ -109,6 +109,23 @@ __device__ __forceinline__ void store_run(T* __restrict__ p, int n, const float 
     }
 }
 
+// The 16 bytes that begin `bytes` (0 .. 15, whole elements) behind the start of a, where b follows a in memory.
+__device__ __forceinline__ uint4 shift16(const uint4& a, const uint4& b, int bytes) {
+    const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    unsigned t[6], u[5];
+#pragma unroll
+    for (int k = 0; k < 6; k++) t[k] = bytes & 8 ? w[k + 2] : w[k];
+#pragma unroll
+    for (int k = 0; k < 5; k++) u[k] = bytes & 4 ? t[k + 1] : t[k];
+    const int bits = (bytes & 3) * 8;
+    return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits),
+                      __funnelshift_r(u[3], u[4], bits));
+}
+
+// elements of T between the last 16-byte boundary and p
+template <class T>
+__device__ __forceinline__ int behind16(const T* p) { return (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T)); }
+
 // every column of a matrix starts on a 16-byte boundary
 inline bool columns16(const void* p, long long ld, int size) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
