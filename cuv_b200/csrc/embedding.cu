@@ -2,6 +2,7 @@
 //   lookup    dst[:, j] = scale * table[:, tok_j]
 //   gradient  dtable[:, v] = factOld * dtable[:, v] + factNew * sum over the j with tok_j = v, ascending, of dout[:, j]
 // A token outside [0, vocab) names no column: the lookup writes zeros for it and the gradient passes over it.
+#include "cluster.cuh"
 #include "typed.cuh"
 
 namespace cuvdia {
@@ -107,15 +108,131 @@ int launch_embedding(void* dst, int ldd, const void* table, int ldt, int type, i
 
 // ---- positions sorted by token -----------------------------------------------------------------------------------
 // A stable least-significant-digit radix sort of the pairs (token, position), a token that names no column becoming
-// `vocab`, the largest key.  Digits of up to 9 bits: two passes for any vocabulary below 2^18.  A pass is three kernels:
-// digit counts of every tile of 4096 pairs, one scan over (digit, tile), and the move of each pair to its place.  Equal
-// tokens stay in ascending position, so the sums below are taken in the same order on every run.
-constexpr int SORT_TILE = 4096, SORT_DIGITS = 512, SORT_THREADS = 256;
+// `vocab`, the largest key.  Digits of up to 9 bits: two passes for any vocabulary below 2^18.  Equal tokens stay in
+// ascending position, so the sums below are taken in the same order on every run.
 
 __device__ __forceinline__ int sort_key(const Tokens& tokens, long long j, int vocab) {
     const long long t = tokens[j];
     return t >= 0 && t < vocab ? (int)t : vocab;
 }
+
+constexpr int SORT_DIGITS = 512;
+
+// Up to 2^17 positions: one cluster of blocks holds all pairs in registers, 32 R consecutive ones a warp, R a lane, and moves
+// them to their places in the blocks' shared memory: one launch, no traffic but tokens in and pairs out.  Per pass a warp ranks
+// its pairs among its earlier ones of the same digit; then come the warps before it in the block, the blocks before it in the
+// cluster, and the smaller digits.
+template <int R>
+__global__ void __launch_bounds__(1024, 1)
+sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit_bits, int* __restrict__ keys_out,
+                    int* __restrict__ pos_out) {
+    constexpr int M = 1024 * R;
+    extern __shared__ unsigned long long pairs[];               // M pairs, then the warps' digit counts, then two rows of digits
+    unsigned short (*hist)[SORT_DIGITS] = reinterpret_cast<unsigned short (*)[SORT_DIGITS]>(pairs + M);
+    int* total = reinterpret_cast<int*>(hist + 32);
+    int* base = total + SORT_DIGITS;
+    __shared__ int warp_sum[16];
+    unsigned rank_in, ranks;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank_in));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << digit_bits;
+    const int g0 = (int)rank_in * M + warp * (32 * R) + lane;
+    int key[R], pos[R], place[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        pos[r] = g0 + r * 32;
+        key[r] = pos[r] < n ? sort_key(tokens, pos[r], vocab) : vocab;          // what fills up the last block stays behind
+    }
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = pass * digit_bits;
+        for (int d = lane; d < SORT_DIGITS / 2; d += 32) reinterpret_cast<unsigned*>(hist[warp])[d] = 0;
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int digit = (key[r] >> shift) & (digits - 1);
+            const unsigned peers = __match_any_sync(0xffffffffu, digit);
+            const int before = hist[warp][digit];
+            place[r] = before + __popc(peers & ((1u << lane) - 1));
+            __syncwarp();
+            if ((peers >> lane) == 1u) hist[warp][digit] = (unsigned short)(before + __popc(peers));     // its highest lane
+            __syncwarp();
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < digits) {
+            int run = 0;
+#pragma unroll 8
+            for (int w = 0; w < 32; w++) { const int v = hist[w][threadIdx.x]; hist[w][threadIdx.x] = (unsigned short)run; run += v; }
+            total[threadIdx.x] = run;
+        }
+        cluster_arrive();
+        cluster_wait();
+        int all = 0, below = 0;
+        if ((int)threadIdx.x < digits)
+            for (unsigned c = 0; c < ranks; c++) {
+                int v;
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(in_block(total + threadIdx.x, c)) : "memory");
+                if (c < rank_in) below += v;
+                all += v;
+            }
+        if (warp < 16) {                                        // exclusive scan over the digits
+            int run = all;
+#pragma unroll
+            for (int s = 1; s < 32; s *= 2) { const int o = __shfl_up_sync(0xffffffffu, run, s); if (lane >= s) run += o; }
+            if (lane == 31) warp_sum[warp] = run;
+            all = run - all;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < digits) {
+            for (int w = 0; w < warp; w++) all += warp_sum[w];
+            base[threadIdx.x] = all + below;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int digit = (key[r] >> shift) & (digits - 1), to = base[digit] + hist[warp][digit] + place[r];
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(pairs + to % M, to / M)),
+                         "l"((unsigned long long)(unsigned)key[r] << 32 | (unsigned)pos[r]) : "memory");
+        }
+        cluster_arrive();
+        cluster_wait();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const unsigned long long p = pairs[warp * (32 * R) + r * 32 + lane];
+            key[r] = (int)(p >> 32); pos[r] = (int)(unsigned)p;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int g = g0 + r * 32;
+        if (g < n) { keys_out[g] = key[r]; pos_out[g] = pos[r]; }
+    }
+}
+
+template <int R>
+static int sort_cluster(int blocks, const Tokens& tokens, int n, int vocab, int passes, int digit_bits, int* keys, int* pos,
+                        cudaStream_t st) {
+    static bool done[64] = {false};
+    const size_t bytes = 1024 * R * 8 + 32 * SORT_DIGITS * 2 + 2 * SORT_DIGITS * 4;
+    int rc = allow_dynamic_smem(sort_cluster_kernel<R>, bytes, done);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = blocks; cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, sort_cluster_kernel<R>, tokens, n, vocab, passes, digit_bits, keys, pos));
+    count_launch();
+    return check_launch("sort_cluster_kernel");
+}
+
+// More positions: a pass is three kernels - digit counts of every tile of 4096 pairs, one scan over (digit, tile), and the
+// move of each pair to its place.
+constexpr int SORT_TILE = 4096, SORT_THREADS = 256;
 
 // the pair at place j of the pass's input: the tokens themselves in the first pass
 template <bool FIRST>
@@ -210,110 +327,228 @@ sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* _
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------
-// The sorted positions are cut into chunks of `len`; a block sums one chunk for one tile of units, in 32 bits and in
-// ascending position.  A token whose positions lie inside the chunk is finished here.  One that reaches over a chunk's
-// border leaves a partial sum: slot 0 of the chunk if the token began in an earlier one, else slot 1; the second kernel
-// adds a token's partial sums in the order of the chunks.
-template <class T, class G, int N, bool ALIGNED>
-__global__ void __launch_bounds__(256)
-embedding_sum_kernel(G* __restrict__ dtable, long long ldt, const T* __restrict__ dout, long long ldo, int units, int vocab,
-                     const int* __restrict__ keys, const int* __restrict__ pos, int n, int len, int tiles,
-                     float* __restrict__ partial, float fnew, float fold) {
-    constexpr int B = 8;                                        // columns in flight
-    __shared__ int skey[130], spos[128];
-    const long long chunk = blockIdx.x / (unsigned)tiles;
-    const int tile = blockIdx.x - (unsigned)chunk * (unsigned)tiles;
-    const long long first = chunk * len;
-    const int count = (int)min((long long)len, n - first);
-    for (int k = threadIdx.x; k < count + 2; k += 256) {        // with the key before and the key after the chunk
-        const long long j = first + k - 1;
-        skey[k] = j >= 0 && j < n ? keys[j] : -1;
-    }
-    for (int k = threadIdx.x; k < count; k += 256) spos[k] = pos[first + k];
-    __syncthreads();
-    const long long u = ((long long)tile * 256 + threadIdx.x) * N;
-    const int nu = (int)max(0LL, min((long long)N, units - u));
-    float acc[N];
+// The sorted positions are cut into chunks of 32; a warp sums one chunk for 256 units, in 32 bits and in ascending position,
+// eight columns in flight.  A token whose positions lie inside the chunk is finished here.  One that reaches over a chunk's
+// border leaves a partial sum: slot 0 of the chunk if the token began in an earlier one, else slot 1; the second kernel adds a
+// token's partial sums, in the order of the chunks or of a fixed split of them.  Behind the blocks that sum come those that
+// write the columns of tokens that do not occur, 32 columns each: stores that fill the memory's time between the loads.
+
+// the eight units of a lane: two runs of four consecutive ones, one of eight, or single ones 32 apart
+template <class T, bool ALIGNED>
+__device__ __forceinline__ int lane_unit(int slice, int e) {
+    const int lane = threadIdx.x & 31;
+    return slice * 256 + (!ALIGNED ? e * 32 + lane : sizeof(T) == 4 ? (e / 4) * 128 + lane * 4 + e % 4 : lane * 8 + e);
+}
+
+// x[e] of the units of a lane to or from a column of C; `units` of them exist.  T lays the lane's units out (see above).
+template <class T, class C, bool ALIGNED>
+__device__ __forceinline__ void store_units(C* to, int slice, int units, const float (&x)[8]) {
+    if constexpr (ALIGNED) {
 #pragma unroll
-    for (int e = 0; e < N; e++) acc[e] = 0.f;
-    bool begun_before = skey[1] == skey[0];
-    for (int k0 = 0; k0 < count; k0 += B) {
-        float x[B][N];
-#pragma unroll
-        for (int b = 0; b < B; b++) {
-            const bool there = k0 + b < count && skey[min(k0 + b, count - 1) + 1] < vocab;
-            load_run<T, N, ALIGNED>(dout + (long long)spos[there ? k0 + b : 0] * ldo + u, there ? nu : 0, x[b]);
-        }
-#pragma unroll
-        for (int b = 0; b < B; b++) {
-            const int k = k0 + b;
-            if (k >= count || skey[k + 1] >= vocab) return;     // the rest names no column
-#pragma unroll
-            for (int e = 0; e < N; e++) acc[e] += x[b][e];
-            const int key = skey[k + 1];
-            const bool goes_on = k + 1 == count && skey[k + 2] == key;
-            if (skey[k + 2] == key && !goes_on) continue;
-            if (!begun_before && !goes_on) {
-                G* to = dtable + (long long)key * ldt + u;
-                float old[N];
-                if (fold != 0.f) load_run<G, N, ALIGNED>(to, nu, old);
-#pragma unroll
-                for (int e = 0; e < N; e++) acc[e] = fold != 0.f ? fold * old[e] + fnew * acc[e] : fnew * acc[e];
-                store_run<G, N, ALIGNED>(to, nu, acc);
+        for (int g = 0; g < 2; g++) {
+            const int u = lane_unit<T, true>(slice, 4 * g);
+            if (u + 4 <= units) {
+                if constexpr (sizeof(C) == 4) *reinterpret_cast<float4*>(to + u) = make_float4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
+                else *reinterpret_cast<uint2*>(to + u) = make_uint2(pack2<C>(x[4 * g], x[4 * g + 1]), pack2<C>(x[4 * g + 2], x[4 * g + 3]));
             } else {
-                float* to = partial + (chunk * 2 + (begun_before ? 0 : 1)) * units + u;
-                store_run<float, N, false>(to, nu, acc);
-            }
-            begun_before = false;
 #pragma unroll
-            for (int e = 0; e < N; e++) acc[e] = 0.f;
+                for (int e = 0; e < 4; e++) if (u + e < units) to[u + e] = from_f32<C>(x[4 * g + e]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int u = lane_unit<T, false>(slice, e);
+            if (u < units) to[u] = from_f32<C>(x[e]);
         }
     }
 }
 
+// A lane's part of a column on its way: as it is in memory (16-byte vectors), or converted (single elements)
+template <class T, bool ALIGNED> struct Part;
+template <class T> struct Part<T, true> {
+    uint4 v[sizeof(T) == 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const T* from, int slice, int units) {
+        constexpr int E = Vec16<T>::N;
+#pragma unroll
+        for (int g = 0; g < 8 / E; g++) {
+            const int u = lane_unit<T, true>(slice, g * E);
+            if (u + E <= units) v[g] = __ldg(reinterpret_cast<const uint4*>(from + u));
+            else {
+                float x[E];
+                load_run<T, E, false>(from + u, max(0, units - u), x);
+                v[g] = pack16<T>(x);
+            }
+        }
+    }
+    __device__ __forceinline__ void add_to(float (&acc)[8]) const {
+        constexpr int E = Vec16<T>::N;
+#pragma unroll
+        for (int g = 0; g < 8 / E; g++) {
+            float x[E];
+            unpack16<T>(v[g], x);
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[g * E + e] += x[e];
+        }
+    }
+};
+template <class T> struct Part<T, false> {
+    T v[8];
+    __device__ __forceinline__ void load(const T* from, int slice, int units) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int u = lane_unit<T, false>(slice, e);
+            v[e] = u < units ? from[u] : from_f32<T>(0.f);
+        }
+    }
+    __device__ __forceinline__ void add_to(float (&acc)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[e] += to_f32(v[e]);
+    }
+};
+
 template <class G>
-__global__ void __launch_bounds__(256)
-embedding_join_kernel(G* __restrict__ dtable, long long ldt, int units, int vocab, const int* __restrict__ keys, int n, int len,
-                      int tiles, const float* __restrict__ partial, float fnew, float fold) {
-    const long long chunk = blockIdx.x / (unsigned)tiles;
-    const int tile = blockIdx.x - (unsigned)chunk * (unsigned)tiles;
-    const long long first = chunk * len, next = first + len;
-    if (next >= n) return;
-    const int key = keys[next - 1];
-    if (key >= vocab || keys[next] != key) return;                                        // no token reaches over
-    if (first > 0 && keys[first] == key && keys[first - 1] == key) return;                // it began in an earlier chunk
-    const long long u = (long long)tile * 256 + threadIdx.x;
-    if (u >= units) return;
-    float acc = partial[(chunk * 2 + 1) * units + u];
-    for (long long c = chunk + 1; c * len < n && keys[c * len] == key; c++) acc += partial[c * 2 * units + u];
-    G* to = dtable + (long long)key * ldt + u;
-    *to = from_f32<G>(fold != 0.f ? fold * to_f32(*to) + fnew * acc : fnew * acc);
+struct GradOut {
+    G* dtable; long long ldt;
+    int units, vocab;
+    const int* keys; const int* pos; int n;
+    float* partial; int pitch;                                  // two rows of `pitch` floats a chunk
+    float fnew, fold;
+};
+
+template <class T, class G, bool ALIGNED>
+__device__ __forceinline__ void finish_column(const GradOut<G>& o, int key, int slice, float (&acc)[8]) {
+    G* to = o.dtable + key * o.ldt;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int u = lane_unit<T, ALIGNED>(slice, e);
+        acc[e] *= o.fnew;
+        if (o.fold != 0.f && u < o.units) acc[e] = o.fold * to_f32(to[u]) + acc[e];
+    }
+    store_units<T, G, ALIGNED>(to, slice, o.units, acc);
 }
 
-// The columns of tokens that do not occur: 32 columns a block.
+// The columns of 32 tokens that do not occur: zeroed or scaled by a block.
 template <class G>
-__global__ void __launch_bounds__(256)
-embedding_rest_kernel(G* __restrict__ dtable, long long ldt, int units, int vocab, const int* __restrict__ keys, int n,
-                      float fold) {
-    __shared__ int occurs[32];
-    const long long v0 = (long long)blockIdx.x * 32;
+__device__ __forceinline__ void rest_columns(const GradOut<G>& o, long long v0, int* occurs) {
     if (threadIdx.x < 32) {
         const long long v = v0 + threadIdx.x;
-        int lo = 0, hi = n;                                     // the first place whose key is not below v
-        while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (keys[mid] < v) lo = mid + 1; else hi = mid; }
-        occurs[threadIdx.x] = v >= vocab || (lo < n && keys[lo] == v);
+        int lo = 0, hi = o.n;                                   // the first place whose key is not below v
+        while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (o.keys[mid] < v) lo = mid + 1; else hi = mid; }
+        occurs[threadIdx.x] = v >= o.vocab || (lo < o.n && o.keys[lo] == v);
     }
     __syncthreads();
     for (int c = 0; c < 32; c++) {
         if (occurs[c]) continue;
-        G* to = dtable + (v0 + c) * ldt;
-        for (long long u = threadIdx.x; u < units; u += 256) to[u] = from_f32<G>(fold == 0.f ? 0.f : fold * to_f32(to[u]));
+        G* to = o.dtable + (v0 + c) * o.ldt;
+        if (o.fold != 0.f) {
+            for (int u = threadIdx.x; u < o.units; u += 256) to[u] = from_f32<G>(o.fold * to_f32(to[u]));
+            continue;
+        }
+        const int head = min(o.units, (int)((16 - (reinterpret_cast<uintptr_t>(to) & 15)) % 16 / sizeof(G)));
+        const int nvec = (o.units - head) / Vec16<G>::N, tail = head + nvec * Vec16<G>::N;
+        uint4* v = reinterpret_cast<uint4*>(to + head);
+        for (int k = threadIdx.x; k < nvec; k += 256) v[k] = make_uint4(0, 0, 0, 0);
+        if ((int)threadIdx.x < head) to[threadIdx.x] = from_f32<G>(0.f);
+        if ((int)threadIdx.x < o.units - tail) to[tail + threadIdx.x] = from_f32<G>(0.f);
+    }
+}
+
+template <class T, class G, bool ALIGNED>
+__global__ void __launch_bounds__(256)
+embedding_sum_kernel(const GradOut<G> o, const T* __restrict__ dout, long long ldo, unsigned sum_blocks, int slices) {
+    constexpr int B = 8;
+    __shared__ int occurs[32];
+    if (blockIdx.x >= sum_blocks) { rest_columns(o, (long long)(blockIdx.x - sum_blocks) * 32, occurs); return; }
+    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long long chunk = item / slices;
+    const int slice = (int)(item - chunk * slices), lane = threadIdx.x & 31;
+    const long long first = chunk * 32;
+    if (first >= o.n) return;
+    const int key = first + lane < o.n ? o.keys[first + lane] : o.vocab, at = first + lane < o.n ? o.pos[first + lane] : 0;
+    const int count = __popc(__ballot_sync(0xffffffffu, key < o.vocab));          // the rest names no column
+    if (count == 0) return;
+    int after = __shfl_down_sync(0xffffffffu, key, 1);
+    if (lane == 31) after = first + 32 < o.n ? o.keys[first + 32] : o.vocab;
+    const unsigned ends = __ballot_sync(0xffffffffu, key != after);
+    bool begun_before = first > 0 && __shfl_sync(0xffffffffu, key, 0) == o.keys[first - 1];
+    float acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) acc[e] = 0.f;
+    for (int k0 = 0; k0 < count; k0 += B) {
+        Part<T, ALIGNED> part[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const long long j = __shfl_sync(0xffffffffu, at, (k0 + b) & 31);
+            if (k0 + b < count) part[b].load(dout + j * ldo, slice, o.units);
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            if (k0 + b >= count) break;
+            part[b].add_to(acc);
+            if (!(ends >> (k0 + b) & 1)) continue;
+            if (begun_before) store_units<T, float, ALIGNED>(o.partial + chunk * 2 * o.pitch, slice, o.units, acc);
+            else finish_column<T, G, ALIGNED>(o, __shfl_sync(0xffffffffu, key, k0 + b), slice, acc);
+            begun_before = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[e] = 0.f;
+        }
+    }
+    if (!(ends >> (count - 1) & 1)) store_units<T, float, ALIGNED>(o.partial + (chunk * 2 + (begun_before ? 0 : 1)) * o.pitch, slice, o.units, acc);
+}
+
+// Adds up the partial sums of the token, if there is one, that begins in a chunk and reaches over its end.  A block takes one
+// chunk and 128 units after the other; with up to eight partial sums a warp takes 128 units of its own, with more the block's
+// warps share the sums of the same 128 units.
+template <class G>
+__global__ void __launch_bounds__(256)
+embedding_join_kernel(const GradOut<G> o) {
+    __shared__ float4 shares[8][32];
+    const long long chunk = blockIdx.x, next = chunk * 32 + 32;
+    if (next >= o.n) return;
+    const int key = o.keys[next - 1];
+    if (key >= o.vocab || o.keys[next] != key) return;                                                     // none reaches over
+    if (chunk > 0 && o.keys[chunk * 32] == key && o.keys[chunk * 32 - 1] == key) return;                   // it began earlier
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int more = 0;                                               // chunks after this one that begin with the token
+    for (;;) {
+        const long long c = (chunk + 1 + more + lane) * 32;
+        const unsigned same = __ballot_sync(0xffffffffu, c < o.n && o.keys[c] == key);
+        const int run = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+        more += run;
+        if (run < 32) break;
+    }
+    const float* own = o.partial + (chunk * 2 + 1) * o.pitch;
+    G* to = o.dtable + key * o.ldt;
+    const bool shared_out = more >= 8;
+    const int begin = shared_out ? (int)((long long)more * warp / 8) : 0, end = shared_out ? (int)((long long)more * (warp + 1) / 8) : more;
+    for (int slice = blockIdx.y; slice * (shared_out ? 128 : 1024) < o.units; slice += gridDim.y) {
+        const int u = (shared_out ? slice * 128 : slice * 1024 + warp * 128) + lane * 4;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](const float4& x) { acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w; };
+        if (u < o.pitch) {
+            if (!shared_out || warp == 0) add(*reinterpret_cast<const float4*>(own + u));
+#pragma unroll 8
+            for (int c = begin; c < end; c++) add(*reinterpret_cast<const float4*>(o.partial + (chunk + 1 + c) * 2 * o.pitch + u));
+        }
+        if (shared_out) {
+            __syncthreads();
+            shares[warp][lane] = acc;
+            __syncthreads();
+            if (warp != 0) continue;
+            for (int w = 1; w < 8; w++) add(shares[w][lane]);
+        }
+        const float x[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (u + e < o.units) to[u + e] = from_f32<G>(o.fold != 0.f ? o.fold * to_f32(to[u + e]) + o.fnew * x[e] : o.fnew * x[e]);
     }
 }
 
 // How the gradient's workspace is laid out, from the sizes alone.
 struct GradLayout {
-    int bits, passes, digit_bits, tiles, len;
+    int bits, passes, digit_bits, tiles, pitch;
+    bool cluster;
     long long chunks;
     long long keys[2], pos[2], counts, partial, bytes;          // byte offsets
 };
@@ -324,16 +559,19 @@ static GradLayout grad_layout(int units, int vocab, int ncols) {
     g.passes = (g.bits + 8) / 9;
     g.digit_bits = (g.bits + g.passes - 1) / g.passes;
     g.tiles = (ncols + SORT_TILE - 1) / SORT_TILE;
-    // Chunks as long as still leave several blocks for each of the GPU's SMs (a longer chunk leaves fewer partial sums).
-    const long long unit_tiles = (units + 1023) / 1024;
-    g.len = 128;
-    while (g.len > 16 && (ncols / g.len) * unit_tiles < 1024) g.len /= 2;
-    g.chunks = ((long long)ncols + g.len - 1) / g.len;
+    g.cluster = ncols <= 131072;
+    g.chunks = ((long long)ncols + 31) / 32;
+    g.pitch = (int)std::min((units + 3LL) / 4 * 4, 2147483644LL);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
-    for (int b = 0; b < 2; b++) { g.keys[b] = take(4LL * ncols); g.pos[b] = take(4LL * ncols); }
-    g.counts = take(4LL * SORT_DIGITS * g.tiles);
-    g.partial = take(4LL * 2 * g.chunks * units);
+    g.keys[0] = take(4LL * ncols);
+    g.pos[0] = take(4LL * ncols);
+    if (!g.cluster) {
+        g.keys[1] = take(4LL * ncols);
+        g.pos[1] = take(4LL * ncols);
+        g.counts = take(4LL * SORT_DIGITS * g.tiles);
+    }
+    g.partial = take(4LL * 2 * g.chunks * g.pitch);
     g.bytes = at;
     return g;
 }
@@ -348,10 +586,22 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     int* keys[2] = {(int*)(ws + g.keys[0]), (int*)(ws + g.keys[1])};
     int* pos[2] = {(int*)(ws + g.pos[0]), (int*)(ws + g.pos[1])};
     int* counts = (int*)(ws + g.counts);
-    float* partial = (float*)(ws + g.partial);
     const Tokens toks = make_tokens(tokens, token_type);
-    int src = 0;
-    for (int p = 0; p < g.passes && ncols > 0; p++) {
+    int src = 0, rc = CUVDIA_OK;
+    if (ncols > 0 && g.cluster) {
+        int blocks = 1, r = 1;
+        while (blocks < 8 && blocks * 1024 < ncols) blocks *= 2;
+        while (blocks * 1024 * r < ncols) r *= 2;
+        switch (r) {
+            case 1: rc = sort_cluster<1>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
+            case 2: rc = sort_cluster<2>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
+            case 4: rc = sort_cluster<4>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
+            case 8: rc = sort_cluster<8>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
+            default: rc = sort_cluster<16>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
+        }
+        if (rc) return rc;
+    }
+    for (int p = 0; p < g.passes && ncols > 0 && !g.cluster; p++) {
         const int shift = p * g.digit_bits, digits = 1 << g.digit_bits;
 #define SORT_GO(F) do {                                                                                                  \
         sort_count_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], ncols, vocab, shift, digits, g.tiles, counts); \
@@ -362,34 +612,36 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
         if (p == 0) SORT_GO(true); else SORT_GO(false);
 #undef SORT_GO
         count_launch(3);
-        int rc = check_launch("sort kernels of embedding_grad");
+        rc = check_launch("sort kernels of embedding_grad");
         if (rc) return rc;
         src = 1 - src;
     }
-    if (fold != 1.f) {
-        const unsigned blocks = (unsigned)(((long long)vocab + 31) / 32);
-        CUVDIA_FLOAT_TYPE(grad_type, (embedding_rest_kernel<T><<<blocks, 256, 0, st>>>((T*)dtable, ldt, units, vocab, keys[src], ncols, fold)));
+    const bool aligned = columns16(dout, ldo, type_size(type)) && columns16(dtable, ldt, type_size(grad_type));
+    const long long slices = ((long long)units + 255) / 256, sum_blocks = (g.chunks * slices + 7) / 8;
+    const long long rest_blocks = fold != 1.f ? ((long long)vocab + 31) / 32 : 0;
+    if (sum_blocks + rest_blocks > 2147483647LL) { set_last_error("embedding_grad: %lld blocks", sum_blocks + rest_blocks); return CUVDIA_ERR_UNSUPPORTED; }
+    if (sum_blocks + rest_blocks > 0) {
+#define SUM_GO(G, A) do {                                                                                                \
+        const GradOut<G> o = {(G*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, fnew, fold}; \
+        embedding_sum_kernel<T, G, A><<<(unsigned)(sum_blocks + rest_blocks), 256, 0, st>>>(o, (const T*)dout, ldo, (unsigned)sum_blocks, (int)slices); \
+    } while (0)
+        CUVDIA_FLOAT_TYPE(type, {
+            if (grad_type == type) { if (aligned) SUM_GO(T, true); else SUM_GO(T, false); }
+            else { if (aligned) SUM_GO(float, true); else SUM_GO(float, false); }
+        });
+#undef SUM_GO
         count_launch();
-        int rc = check_launch("embedding_rest_kernel");
+        rc = check_launch("embedding_sum_kernel");
         if (rc) return rc;
     }
-    if (ncols == 0) return CUVDIA_OK;
-    const bool aligned = columns16(dout, ldo, type_size(type)) && columns16(dtable, ldt, type_size(grad_type));
-    const int n = aligned ? 16 / type_size(type) : 1;
-    const long long tiles = ((long long)units + 256 * n - 1) / (256 * n), blocks = g.chunks * tiles;
-    const long long jtiles = ((long long)units + 255) / 256, jblocks = g.chunks * jtiles;
-    if (jblocks > 2147483647LL || blocks > 2147483647LL) { set_last_error("embedding_grad: %lld blocks", jblocks); return CUVDIA_ERR_UNSUPPORTED; }
-#define SUM_GO(G, N, A) embedding_sum_kernel<T, G, N, A><<<(unsigned)blocks, 256, 0, st>>>((G*)dtable, ldt, (const T*)dout, ldo, \
-    units, vocab, keys[src], pos[src], ncols, g.len, (int)tiles, partial, fnew, fold)
-    CUVDIA_FLOAT_TYPE(type, {
-        if (grad_type == type) { if (aligned) SUM_GO(T, Vec16<T>::N, true); else SUM_GO(T, 1, false); }
-        else { if (aligned) SUM_GO(float, Vec16<T>::N, true); else SUM_GO(float, 1, false); }
+    if (g.chunks < 2) return CUVDIA_OK;
+    const unsigned y = (unsigned)std::max(1LL, std::min(((long long)units + 127) / 128, 2048 / g.chunks));
+    CUVDIA_FLOAT_TYPE(grad_type, {
+        const GradOut<T> o = {(T*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, fnew, fold};
+        embedding_join_kernel<T><<<dim3((unsigned)(g.chunks - 1), y), 256, 0, st>>>(o);
     });
-#undef SUM_GO
-    CUVDIA_FLOAT_TYPE(grad_type, (embedding_join_kernel<T><<<(unsigned)jblocks, 256, 0, st>>>((T*)dtable, ldt, units, vocab,
-        keys[src], ncols, g.len, (int)jtiles, partial, fnew, fold)));
-    count_launch(2);
-    return check_launch("embedding_sum_kernel");
+    count_launch();
+    return check_launch("embedding_join_kernel");
 }
 
 }  // namespace cuvdia

@@ -8,6 +8,7 @@
 // M, s and t come from one pass: a running maximum, and sums that are rescaled by 2^(c * (old M - new M)) when it grows.
 #include <type_traits>
 
+#include "cluster.cuh"
 #include "typed.cuh"
 
 namespace cuvdia {
@@ -352,14 +353,6 @@ __device__ __forceinline__ void add_chunk(Sums& a, const uint4* v, int step, flo
     if (ENT) a.t = __fadd2_rn(a.t, t);
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// the address, in the cluster's first block, of the variable that this block sees at p
-__device__ __forceinline__ unsigned in_first_block(const void* p) {
-    unsigned a = (unsigned)__cvta_generic_to_shared(p), r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
-    return r;
-}
 __device__ __forceinline__ void store_remote(unsigned to, unsigned v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
 }
@@ -534,10 +527,10 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
         cluster_wait();
         if (warp == 0) {
             if (lane == 0) {
-                const unsigned to = in_first_block(&part_stats[part]);
+                const unsigned to = in_block(&part_stats[part], 0);
                 store_remote(to, __float_as_uint(st.m)); store_remote(to + 4, __float_as_uint(st.s)); store_remote(to + 8, __float_as_uint(st.t));
             }
-            if (TOP) store_remote(in_first_block(&part_lists[part][lane]), list);
+            if (TOP) store_remote(in_block(&part_lists[part][lane], 0), list);
         }
         cluster_arrive();
         cluster_wait();
