@@ -125,7 +125,7 @@ constexpr int SORT_DIGITS = 512;
 template <int R>
 __global__ void __launch_bounds__(1024, 1)
 sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit_bits, int* __restrict__ keys_out,
-                    int* __restrict__ pos_out) {
+                    int* __restrict__ pos_out, int* __restrict__ joins) {
     constexpr int M = 1024 * R;
     extern __shared__ unsigned long long pairs[];               // M pairs, then the warps' digit counts, then two rows of digits
     unsigned short (*hist)[SORT_DIGITS] = reinterpret_cast<unsigned short (*)[SORT_DIGITS]>(pairs + M);
@@ -137,6 +137,7 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << digit_bits;
     const int g0 = (int)rank_in * M + warp * (32 * R) + lane;
+    if (rank_in == 0 && threadIdx.x < 2) joins[threadIdx.x] = 0;
     int key[R], pos[R], place[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -187,30 +188,32 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
             base[threadIdx.x] = all + below;
         }
         __syncthreads();
+        const bool last = pass + 1 == passes;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int digit = (key[r] >> shift) & (digits - 1), to = base[digit] + hist[warp][digit] + place[r];
-            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(pairs + to % M, to / M)),
-                         "l"((unsigned long long)(unsigned)key[r] << 32 | (unsigned)pos[r]) : "memory");
+            if (!last) {
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(pairs + to % M, to / M)),
+                             "l"((unsigned long long)(unsigned)key[r] << 32 | (unsigned)pos[r]) : "memory");
+            } else if (to < n) {
+                keys_out[to] = key[r];
+                pos_out[to] = pos[r];
+            }
         }
-        cluster_arrive();
+        cluster_arrive();                                       // after the last pass too: no block leaves while its counts are read
         cluster_wait();
+        if (last) break;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const unsigned long long p = pairs[warp * (32 * R) + r * 32 + lane];
             key[r] = (int)(p >> 32); pos[r] = (int)(unsigned)p;
         }
     }
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int g = g0 + r * 32;
-        if (g < n) { keys_out[g] = key[r]; pos_out[g] = pos[r]; }
-    }
 }
 
 template <int R>
 static int sort_cluster(int blocks, const Tokens& tokens, int n, int vocab, int passes, int digit_bits, int* keys, int* pos,
-                        cudaStream_t st) {
+                        int* joins, cudaStream_t st) {
     static bool done[64] = {false};
     const size_t bytes = 1024 * R * 8 + 32 * SORT_DIGITS * 2 + 2 * SORT_DIGITS * 4;
     int rc = allow_dynamic_smem(sort_cluster_kernel<R>, bytes, done);
@@ -225,7 +228,7 @@ static int sort_cluster(int blocks, const Tokens& tokens, int n, int vocab, int 
     cluster.val.clusterDim.x = blocks; cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = 1;
-    CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, sort_cluster_kernel<R>, tokens, n, vocab, passes, digit_bits, keys, pos));
+    CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, sort_cluster_kernel<R>, tokens, n, vocab, passes, digit_bits, keys, pos, joins));
     count_launch();
     return check_launch("sort_cluster_kernel");
 }
@@ -258,8 +261,9 @@ sort_count_kernel(const Tokens tokens, const int* __restrict__ keys, int n, int 
 }
 
 // exclusive scan of `n` counts in place, one block
-__global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ counts, long long n) {
+__global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ counts, long long n, int* __restrict__ joins) {
     __shared__ int warp_sum[32];
+    if (threadIdx.x < 2) joins[threadIdx.x] = 0;
     const long long per = (n + 1023) / 1024, first = per * threadIdx.x, last = min(n, first + per);
     int sum = 0;
     for (long long k = first; k < last; k++) sum += counts[k];
@@ -332,6 +336,8 @@ sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* _
 // border leaves a partial sum: slot 0 of the chunk if the token began in an earlier one, else slot 1; the second kernel adds a
 // token's partial sums, in the order of the chunks or of a fixed split of them.  Behind the blocks that sum come those that
 // write the columns of tokens that do not occur, 32 columns each: stores that fill the memory's time between the loads.
+
+constexpr int LONG_JOIN = 8;            // more partial sums than this are shared out among a block's warps
 
 // the eight units of a lane: two runs of four consecutive ones, one of eight, or single ones 32 apart
 template <class T, bool ALIGNED>
@@ -413,6 +419,7 @@ struct GradOut {
     int units, vocab;
     const int* keys; const int* pos; int n;
     float* partial; int pitch;                                  // two rows of `pitch` floats a chunk
+    int* joins; int chunks;                                     // numbers of short and long joins, then their chunks from both ends
     float fnew, fold;
 };
 
@@ -438,19 +445,23 @@ __device__ __forceinline__ void rest_columns(const GradOut<G>& o, long long v0, 
         occurs[threadIdx.x] = v >= o.vocab || (lo < o.n && o.keys[lo] == v);
     }
     __syncthreads();
-    for (int c = 0; c < 32; c++) {
+    // a warp a column: a whole block would be half empty on short ones
+    const int lane = threadIdx.x & 31;
+    for (int c = threadIdx.x >> 5; c < 32; c += 8) {
         if (occurs[c]) continue;
         G* to = o.dtable + (v0 + c) * o.ldt;
         if (o.fold != 0.f) {
-            for (int u = threadIdx.x; u < o.units; u += 256) to[u] = from_f32<G>(o.fold * to_f32(to[u]));
+#pragma unroll 4
+            for (int u = lane; u < o.units; u += 32) to[u] = from_f32<G>(o.fold * to_f32(to[u]));
             continue;
         }
         const int head = min(o.units, (int)((16 - (reinterpret_cast<uintptr_t>(to) & 15)) % 16 / sizeof(G)));
         const int nvec = (o.units - head) / Vec16<G>::N, tail = head + nvec * Vec16<G>::N;
         uint4* v = reinterpret_cast<uint4*>(to + head);
-        for (int k = threadIdx.x; k < nvec; k += 256) v[k] = make_uint4(0, 0, 0, 0);
-        if ((int)threadIdx.x < head) to[threadIdx.x] = from_f32<G>(0.f);
-        if ((int)threadIdx.x < o.units - tail) to[tail + threadIdx.x] = from_f32<G>(0.f);
+#pragma unroll 4
+        for (int k = lane; k < nvec; k += 32) v[k] = make_uint4(0, 0, 0, 0);
+        if (lane < head) to[lane] = from_f32<G>(0.f);
+        if (lane < o.units - tail) to[tail + lane] = from_f32<G>(0.f);
     }
 }
 
@@ -494,54 +505,71 @@ embedding_sum_kernel(const GradOut<G> o, const T* __restrict__ dout, long long l
             for (int e = 0; e < 8; e++) acc[e] = 0.f;
         }
     }
-    if (!(ends >> (count - 1) & 1)) store_units<T, float, ALIGNED>(o.partial + (chunk * 2 + (begun_before ? 0 : 1)) * o.pitch, slice, o.units, acc);
+    if (ends >> (count - 1) & 1) return;
+    store_units<T, float, ALIGNED>(o.partial + (chunk * 2 + (begun_before ? 0 : 1)) * o.pitch, slice, o.units, acc);
+    if (!begun_before && slice == 0 && lane == 31) {            // this chunk's last token is to be joined
+        const long long far = first + (LONG_JOIN + 1) * 32;
+        const bool is_long = far < o.n && o.keys[far] == key;
+        const int place = atomicAdd(&o.joins[is_long], 1);
+        o.joins[2 + (is_long ? o.chunks - 1 - place : place)] = (int)chunk;
+    }
 }
 
-// Adds up the partial sums of the token, if there is one, that begins in a chunk and reaches over its end.  A block takes one
-// chunk and 128 units after the other; with up to eight partial sums a warp takes 128 units of its own, with more the block's
-// warps share the sums of the same 128 units.
+// Adds up the partial sums of the tokens that reach over a chunk's end, from the list of the chunks where they begin (the list's
+// order changes nothing: every sum has its own place).  128 units at a time, by one warp, or by a block whose warps share out the
+// partial sums where they are many.
 template <class G>
 __global__ void __launch_bounds__(256)
 embedding_join_kernel(const GradOut<G> o) {
     __shared__ float4 shares[8][32];
-    const long long chunk = blockIdx.x, next = chunk * 32 + 32;
-    if (next >= o.n) return;
-    const int key = o.keys[next - 1];
-    if (key >= o.vocab || o.keys[next] != key) return;                                                     // none reaches over
-    if (chunk > 0 && o.keys[chunk * 32] == key && o.keys[chunk * 32 - 1] == key) return;                   // it began earlier
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int more = 0;                                               // chunks after this one that begin with the token
-    for (;;) {
-        const long long c = (chunk + 1 + more + lane) * 32;
-        const unsigned same = __ballot_sync(0xffffffffu, c < o.n && o.keys[c] == key);
-        const int run = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
-        more += run;
-        if (run < 32) break;
-    }
-    const float* own = o.partial + (chunk * 2 + 1) * o.pitch;
-    G* to = o.dtable + key * o.ldt;
-    const bool shared_out = more >= 8;
-    const int begin = shared_out ? (int)((long long)more * warp / 8) : 0, end = shared_out ? (int)((long long)more * (warp + 1) / 8) : more;
-    for (int slice = blockIdx.y; slice * (shared_out ? 128 : 1024) < o.units; slice += gridDim.y) {
-        const int u = (shared_out ? slice * 128 : slice * 1024 + warp * 128) + lane * 4;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](const float4& x) { acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w; };
-        if (u < o.pitch) {
-            if (!shared_out || warp == 0) add(*reinterpret_cast<const float4*>(own + u));
-#pragma unroll 8
-            for (int c = begin; c < end; c++) add(*reinterpret_cast<const float4*>(o.partial + (chunk + 1 + c) * 2 * o.pitch + u));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slices = (o.units + 127) / 128;
+    // chunks after this one that begin with the token
+    auto followers = [&](int chunk, int key) {
+        int more = 0;
+        for (;;) {
+            const long long c = ((long long)chunk + 1 + more + lane) * 32;
+            const unsigned same = __ballot_sync(0xffffffffu, c < o.n && o.keys[c] == key);
+            if (same != 0xffffffffu) return more + __ffs(~same) - 1;
+            more += 32;
         }
-        if (shared_out) {
-            __syncthreads();
-            shares[warp][lane] = acc;
-            __syncthreads();
-            if (warp != 0) continue;
-            for (int w = 1; w < 8; w++) add(shares[w][lane]);
-        }
+    };
+    auto add = [](float4& acc, const float4& x) { acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w; };
+    auto finish = [&](int key, int u, const float4& acc) {
+        G* to = o.dtable + key * o.ldt;
         const float x[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (u + e < o.units) to[u + e] = from_f32<G>(o.fold != 0.f ? o.fold * to_f32(to[u + e]) + o.fnew * x[e] : o.fnew * x[e]);
+    };
+    const long long n_long = (long long)o.joins[1] * slices, n_short = (long long)o.joins[0] * slices;
+    for (long long item = blockIdx.x; item < n_long; item += gridDim.x) {
+        const int chunk = o.joins[2 + o.chunks - 1 - (int)(item / slices)], u = (int)(item % slices) * 128 + lane * 4;
+        const int key = o.keys[(long long)chunk * 32 + 31], more = followers(chunk, key);
+        const float* row = o.partial + ((long long)chunk * 2 + 2) * o.pitch + u;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u < o.pitch) {
+            if (warp == 0) add(acc, *reinterpret_cast<const float4*>(row - o.pitch));
+            const int end = (int)((long long)more * (warp + 1) / 8);
+#pragma unroll 8
+            for (int c = (int)((long long)more * warp / 8); c < end; c++) add(acc, *reinterpret_cast<const float4*>(row + (long long)c * 2 * o.pitch));
+        }
+        __syncthreads();
+        shares[warp][lane] = acc;
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < 8; w++) add(acc, shares[w][lane]);
+            finish(key, u, acc);
+        }
+    }
+    for (long long item = (long long)blockIdx.x * 8 + warp; item < n_short; item += (long long)gridDim.x * 8) {
+        const int chunk = o.joins[2 + (int)(item / slices)], u = (int)(item % slices) * 128 + lane * 4;
+        const int key = o.keys[(long long)chunk * 32 + 31], more = followers(chunk, key);
+        const float* row = o.partial + ((long long)chunk * 2 + 2) * o.pitch + u;
+        if (u >= o.pitch) continue;
+        float4 acc = *reinterpret_cast<const float4*>(row - o.pitch);
+#pragma unroll 8
+        for (int c = 0; c < more; c++) add(acc, *reinterpret_cast<const float4*>(row + (long long)c * 2 * o.pitch));
+        finish(key, u, acc);
     }
 }
 
@@ -550,7 +578,7 @@ struct GradLayout {
     int bits, passes, digit_bits, tiles, pitch;
     bool cluster;
     long long chunks;
-    long long keys[2], pos[2], counts, partial, bytes;          // byte offsets
+    long long keys[2], pos[2], counts, joins, partial, bytes;          // byte offsets
 };
 
 static GradLayout grad_layout(int units, int vocab, int ncols) {
@@ -571,6 +599,7 @@ static GradLayout grad_layout(int units, int vocab, int ncols) {
         g.pos[1] = take(4LL * ncols);
         g.counts = take(4LL * SORT_DIGITS * g.tiles);
     }
+    g.joins = take(4LL * (2 + g.chunks));
     g.partial = take(4LL * 2 * g.chunks * g.pitch);
     g.bytes = at;
     return g;
@@ -586,6 +615,7 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     int* keys[2] = {(int*)(ws + g.keys[0]), (int*)(ws + g.keys[1])};
     int* pos[2] = {(int*)(ws + g.pos[0]), (int*)(ws + g.pos[1])};
     int* counts = (int*)(ws + g.counts);
+    int* joins = (int*)(ws + g.joins);
     const Tokens toks = make_tokens(tokens, token_type);
     int src = 0, rc = CUVDIA_OK;
     if (ncols > 0 && g.cluster) {
@@ -593,11 +623,11 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
         while (blocks < 8 && blocks * 1024 < ncols) blocks *= 2;
         while (blocks * 1024 * r < ncols) r *= 2;
         switch (r) {
-            case 1: rc = sort_cluster<1>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
-            case 2: rc = sort_cluster<2>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
-            case 4: rc = sort_cluster<4>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
-            case 8: rc = sort_cluster<8>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
-            default: rc = sort_cluster<16>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], st); break;
+            case 1: rc = sort_cluster<1>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], joins, st); break;
+            case 2: rc = sort_cluster<2>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], joins, st); break;
+            case 4: rc = sort_cluster<4>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], joins, st); break;
+            case 8: rc = sort_cluster<8>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], joins, st); break;
+            default: rc = sort_cluster<16>(blocks, toks, ncols, vocab, g.passes, g.digit_bits, keys[0], pos[0], joins, st); break;
         }
         if (rc) return rc;
     }
@@ -605,7 +635,7 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
         const int shift = p * g.digit_bits, digits = 1 << g.digit_bits;
 #define SORT_GO(F) do {                                                                                                  \
         sort_count_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], ncols, vocab, shift, digits, g.tiles, counts); \
-        sort_scan_kernel<<<1, 1024, 0, st>>>(counts, (long long)digits * g.tiles);                                       \
+        sort_scan_kernel<<<1, 1024, 0, st>>>(counts, (long long)digits * g.tiles, joins);                                \
         sort_move_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], pos[src], ncols, vocab, shift, digits,    \
                                                               g.tiles, counts, keys[1 - src], pos[1 - src]);             \
     } while (0)
@@ -622,7 +652,7 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     if (sum_blocks + rest_blocks > 2147483647LL) { set_last_error("embedding_grad: %lld blocks", sum_blocks + rest_blocks); return CUVDIA_ERR_UNSUPPORTED; }
     if (sum_blocks + rest_blocks > 0) {
 #define SUM_GO(G, A) do {                                                                                                \
-        const GradOut<G> o = {(G*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, fnew, fold}; \
+        const GradOut<G> o = {(G*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, joins, (int)g.chunks, fnew, fold}; \
         embedding_sum_kernel<T, G, A><<<(unsigned)(sum_blocks + rest_blocks), 256, 0, st>>>(o, (const T*)dout, ldo, (unsigned)sum_blocks, (int)slices); \
     } while (0)
         CUVDIA_FLOAT_TYPE(type, {
@@ -635,10 +665,10 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
         if (rc) return rc;
     }
     if (g.chunks < 2) return CUVDIA_OK;
-    const unsigned y = (unsigned)std::max(1LL, std::min(((long long)units + 127) / 128, 2048 / g.chunks));
+    const unsigned join_blocks = (unsigned)std::min((g.chunks - 1) * (((long long)units + 127) / 128), 4LL * sm_count());
     CUVDIA_FLOAT_TYPE(grad_type, {
-        const GradOut<T> o = {(T*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, fnew, fold};
-        embedding_join_kernel<T><<<dim3((unsigned)(g.chunks - 1), y), 256, 0, st>>>(o);
+        const GradOut<T> o = {(T*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, joins, (int)g.chunks, fnew, fold};
+        embedding_join_kernel<T><<<join_blocks, 256, 0, st>>>(o);
     });
     count_launch();
     return check_launch("embedding_join_kernel");
