@@ -118,6 +118,17 @@ __device__ __forceinline__ int sort_key(const Tokens& tokens, long long j, int v
 
 constexpr int SORT_DIGITS = 512;
 
+// the lanes of the warp whose digit is the same, from one vote a bit (match.any takes several times as long)
+__device__ __forceinline__ unsigned same_digit(int digit, int bits) {
+    unsigned peers = 0xffffffffu;
+    for (int b = 0; b < bits; b++) {
+        const bool set = digit >> b & 1;
+        const unsigned votes = __ballot_sync(0xffffffffu, set);
+        peers &= set ? votes : ~votes;
+    }
+    return peers;
+}
+
 // Up to 2^17 positions: one cluster of blocks holds all pairs in registers, 32 R consecutive ones a warp, R a lane, and moves
 // them to their places in the blocks' shared memory: one launch, no traffic but tokens in and pairs out.  Per pass a warp ranks
 // its pairs among its earlier ones of the same digit; then come the warps before it in the block, the blocks before it in the
@@ -151,7 +162,7 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int digit = (key[r] >> shift) & (digits - 1);
-            const unsigned peers = __match_any_sync(0xffffffffu, digit);
+            const unsigned peers = same_digit(digit, digit_bits);
             const int before = hist[warp][digit];
             place[r] = before + __popc(peers & ((1u << lane) - 1));
             __syncwarp();
@@ -288,8 +299,9 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ count
 template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* __restrict__ pos, int n, int vocab,
-                 int shift, int digits, int tiles, const int* __restrict__ counts, int* __restrict__ keys_out,
+                 int shift, int digit_bits, int tiles, const int* __restrict__ counts, int* __restrict__ keys_out,
                  int* __restrict__ pos_out) {
+    const int digits = 1 << digit_bits;
     constexpr int WARPS = SORT_THREADS / 32, PER = SORT_TILE / SORT_THREADS;
     __shared__ int hist[WARPS][SORT_DIGITS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -308,7 +320,7 @@ sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* _
     for (int r = 0; r < PER; r++) {
         const bool valid = first + r * 32 < n;
         const int digit = valid ? (key[r] >> shift) & (digits - 1) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, digit);
+        const unsigned peers = same_digit(valid ? digit : digits, digit_bits + 1);       // a digit of its own for what is not there
         rank[r] = valid ? hist[warp][digit] + __popc(peers & ((1u << lane) - 1)) : 0;
         __syncwarp();
         if (valid && (peers >> lane) == 1u) hist[warp][digit] += __popc(peers);       // the highest lane of the digit
@@ -636,7 +648,7 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
 #define SORT_GO(F) do {                                                                                                  \
         sort_count_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], ncols, vocab, shift, digits, g.tiles, counts); \
         sort_scan_kernel<<<1, 1024, 0, st>>>(counts, (long long)digits * g.tiles, joins);                                \
-        sort_move_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], pos[src], ncols, vocab, shift, digits,    \
+        sort_move_kernel<F><<<g.tiles, SORT_THREADS, 0, st>>>(toks, keys[src], pos[src], ncols, vocab, shift, g.digit_bits, \
                                                               g.tiles, counts, keys[1 - src], pos[1 - src]);             \
     } while (0)
         if (p == 0) SORT_GO(true); else SORT_GO(false);

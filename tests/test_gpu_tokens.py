@@ -130,7 +130,7 @@ def test_embedding_grad(kind, grad, units, ld, offset, vocab, ncols):
         outside_untouched(buf, dtable)
 
 
-@pytest.mark.parametrize("ncols", [31, 4095, 4097, 8192, 8193, 20000, 70001])
+@pytest.mark.parametrize("ncols", [31, 1024, 1025, 4095, 4097, 8192, 8193, 16384, 20000, 32769, 70001, 131072, 131073, 300001])
 @pytest.mark.parametrize("vocab", [2, 511, 512, 131071, 300007])
 def test_embedding_grad_sums_whole_numbers_exactly(ncols, vocab):
     """Whole numbers whose sums stay below 2^24: equality, whatever the order; text-like frequencies, so that single
