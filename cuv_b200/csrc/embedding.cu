@@ -121,7 +121,9 @@ constexpr int SORT_DIGITS = 512;
 // the lanes of the warp whose digit is the same, from one vote a bit (match.any takes several times as long)
 __device__ __forceinline__ unsigned same_digit(int digit, int bits) {
     unsigned peers = 0xffffffffu;
-    for (int b = 0; b < bits; b++) {
+#pragma unroll
+    for (int b = 0; b < 10; b++) {
+        if (b >= bits) break;
         const bool set = digit >> b & 1;
         const unsigned votes = __ballot_sync(0xffffffffu, set);
         peers &= set ? votes : ~votes;
@@ -179,13 +181,18 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
         cluster_arrive();
         cluster_wait();
         int all = 0, below = 0;
-        if ((int)threadIdx.x < digits)
-            for (unsigned c = 0; c < ranks; c++) {
-                int v;
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(in_block(total + threadIdx.x, c)) : "memory");
-                if (c < rank_in) below += v;
-                all += v;
+        if ((int)threadIdx.x < digits) {
+            int v[8];                                           // all on their way before the first is added
+#pragma unroll
+            for (unsigned c = 0; c < 8; c++) {
+                v[c] = 0;
+                if (c < ranks) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[c]) : "r"(in_block(total + threadIdx.x, c)) : "memory");
             }
+#pragma unroll
+            for (unsigned c = 0; c < 8; c++) { all += v[c]; if (c < rank_in) below += v[c]; }
+        }
+        const bool last = pass + 1 == passes;
+        if (last) cluster_arrive_relaxed();                     // this block has read the others' counts: they may leave
         if (warp < 16) {                                        // exclusive scan over the digits
             int run = all;
 #pragma unroll
@@ -199,7 +206,6 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
             base[threadIdx.x] = all + below;
         }
         __syncthreads();
-        const bool last = pass + 1 == passes;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int digit = (key[r] >> shift) & (digits - 1), to = base[digit] + hist[warp][digit] + place[r];
@@ -211,15 +217,16 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
                 pos_out[to] = pos[r];
             }
         }
-        cluster_arrive();                                       // after the last pass too: no block leaves while its counts are read
-        cluster_wait();
         if (last) break;
+        cluster_arrive();
+        cluster_wait();
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const unsigned long long p = pairs[warp * (32 * R) + r * 32 + lane];
             key[r] = (int)(p >> 32); pos[r] = (int)(unsigned)p;
         }
     }
+    cluster_wait();                                             // a block's counts stay until the others have read them
 }
 
 template <int R>
