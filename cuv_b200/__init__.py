@@ -650,7 +650,7 @@ def embedding(dst, table, tokens, scale=1.0):
     tt = _token_type(tokens, ncols, table)
     if ncols:
         _call(table, "cuvdia_embedding", dst.data_ptr(), ldd, table.data_ptr(), ldt, code, units, vocab, tokens.data_ptr(), tt,
-              ncols, scale)
+              ncols, float(scale))
     return dst
 
 
@@ -673,7 +673,7 @@ def embedding_grad(dtable, tokens, dout, factNew=1.0, factOld=0.0):
     _capi.check(_capi.lib().cuvdia_embedding_grad_workspace(units, vocab, ncols, ctypes.byref(need)))
     work = torch.empty(need.value, dtype=torch.uint8, device=dout.device)
     _call(dout, "cuvdia_embedding_grad", dtable.data_ptr(), ldt, grad_code, dout.data_ptr(), ldo, code, units, vocab,
-          tokens.data_ptr(), tt, ncols, factNew, factOld, work.data_ptr(), need.value)
+          tokens.data_ptr(), tt, ncols, float(factNew), float(factOld), work.data_ptr(), need.value)
     return dtable
 
 
@@ -687,8 +687,8 @@ def dropout(dst, src, p, seed, step=0, col0=0, which=0, residual=None):
     ldr = _matrix(residual, "residual", src, shape, dtype)[0] if residual is not None else 0
     rows, ncols = shape
     if ncols:
-        _call(src, "cuvdia_dropout", dst.data_ptr(), ldd, src.data_ptr(), lds, _address(residual), ldr, code, rows, ncols, p,
-              ctypes.byref(_capi.Draw(seed, step, col0)), which)
+        _call(src, "cuvdia_dropout", dst.data_ptr(), ldd, src.data_ptr(), lds, _address(residual), ldr, code, rows, ncols, float(p),
+              ctypes.byref(_capi.Draw(int(seed), int(step), int(col0))), int(which))
     return dst
 
 
@@ -711,6 +711,7 @@ def token_logprob(logits, tokens=None, scale=1.0, entropy=False, top=0):
     ld, code = _matrix(logits, "logits")
     vocab, ncols = logits.shape
     tt = _token_type(tokens, ncols, logits) if tokens is not None else 0
+    top = int(top)
     if not 0 <= top <= 32:
         _invalid("0 <= top <= 32")
     device = logits.device
@@ -724,7 +725,7 @@ def token_logprob(logits, tokens=None, scale=1.0, entropy=False, top=0):
         top_logp = torch.empty_strided((top, ncols), (1, top), dtype=torch.float32, device=device)
         top_index = torch.empty_strided((top, ncols), (1, top), dtype=torch.int32, device=device)
     if ncols:
-        _call(logits, "cuvdia_token_logprob", logits.data_ptr(), ld, code, vocab, ncols, _address(tokens), tt, scale,
+        _call(logits, "cuvdia_token_logprob", logits.data_ptr(), ld, code, vocab, ncols, _address(tokens), tt, float(scale),
               _address(logp), lse.data_ptr(), _address(ent), top, _address(top_logp), _address(top_index))
     return TokenLogprob(logp, lse, ent, top_logp, top_index)
 
@@ -743,5 +744,5 @@ def token_logprob_grad(dlogits, logits, lse, tokens=None, dlogp=None, entropy=No
             _vector(t, name, ncols, logits)
     if ncols:
         _call(logits, "cuvdia_token_logprob_grad", dlogits.data_ptr(), ldd, logits.data_ptr(), ld, code, vocab, ncols,
-              _address(tokens), tt, scale, lse.data_ptr(), _address(dlogp), _address(entropy), _address(dentropy))
+              _address(tokens), tt, float(scale), lse.data_ptr(), _address(dlogp), _address(entropy), _address(dentropy))
     return dlogits

@@ -451,7 +451,7 @@ int cuvdia_embedding(void* dst, int ldd, const void* table, int ldt, int type, i
     CUVDIA_REQUIRE(is_float_type(type));
     CUVDIA_REQUIRE(is_token_type(token_type));
     CUVDIA_REQUIRE(whole_elements(dst, type) && whole_elements(table, type) && whole_elements(tokens, token_type));
-    CUVDIA_REQUIRE(units > 0 && vocab > 0 && ncols >= 0);
+    CUVDIA_REQUIRE(units > 0 && units <= (1 << 30) && vocab > 0 && ncols >= 0);
     CUVDIA_REQUIRE(ldd >= units && ldt >= units);
     if (ncols == 0) return CUVDIA_OK;
     return launch_embedding(dst, ldd, table, ldt, type, units, vocab, tokens, token_type, ncols, scale, (cudaStream_t)stream);
@@ -459,7 +459,7 @@ int cuvdia_embedding(void* dst, int ldd, const void* table, int ldt, int type, i
 
 int cuvdia_embedding_grad_workspace(int units, int vocab, int ncols, long long* bytes) {
     CUVDIA_REQUIRE(bytes != nullptr);
-    CUVDIA_REQUIRE(units > 0 && vocab > 0 && ncols >= 0 && ncols <= (1 << 30));
+    CUVDIA_REQUIRE(units > 0 && units <= (1 << 30) && vocab > 0 && ncols >= 0 && ncols <= (1 << 30));
     *bytes = embedding_grad_bytes(units, vocab, ncols);
     return CUVDIA_OK;
 }
@@ -471,7 +471,7 @@ int cuvdia_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     CUVDIA_REQUIRE(is_float_type(type));
     CUVDIA_REQUIRE(grad_type == type || grad_type == CUVDIA_T_F32);
     CUVDIA_REQUIRE(is_token_type(token_type));
-    CUVDIA_REQUIRE(units > 0 && vocab > 0 && ncols >= 0 && ncols <= (1 << 30));
+    CUVDIA_REQUIRE(units > 0 && units <= (1 << 30) && vocab > 0 && ncols >= 0 && ncols <= (1 << 30));
     CUVDIA_REQUIRE(ldt >= units);
     CUVDIA_REQUIRE(whole_elements(dtable, grad_type));
     if (ncols > 0) {
@@ -490,7 +490,7 @@ int cuvdia_dropout(void* dst, int ldd, const void* src, int lds, const void* res
     CUVDIA_REQUIRE(dst != nullptr && src != nullptr && draw != nullptr);
     CUVDIA_REQUIRE(is_float_type(type));
     CUVDIA_REQUIRE(whole_elements(dst, type) && whole_elements(src, type) && whole_elements(residual, type));
-    CUVDIA_REQUIRE(rows > 0 && ncols >= 0);
+    CUVDIA_REQUIRE(rows > 0 && rows <= (1 << 30) && ncols >= 0);
     CUVDIA_REQUIRE(ldd >= rows && lds >= rows && (residual == nullptr || ldr >= rows));
     CUVDIA_REQUIRE(p >= 0.f && p <= 1.f);
     CUVDIA_REQUIRE(which >= 0 && which < 65536);
@@ -514,6 +514,8 @@ int cuvdia_token_logprob(const void* logits, int ld, int type, int vocab, int nc
     CUVDIA_REQUIRE(top >= 0 && top <= 32);
     CUVDIA_REQUIRE(top == 0 || (top_logp != nullptr && top_index != nullptr));
     CUVDIA_REQUIRE(logp != nullptr || lse != nullptr || entropy != nullptr || top > 0);
+    CUVDIA_REQUIRE(whole_elements(logp, CUVDIA_T_F32) && whole_elements(lse, CUVDIA_T_F32) && whole_elements(entropy, CUVDIA_T_F32));
+    CUVDIA_REQUIRE(whole_elements(top_logp, CUVDIA_T_F32) && whole_elements(top_index, CUVDIA_T_I32));
     if (ncols == 0) return CUVDIA_OK;
     return launch_token_logprob(logits, ld, type, vocab, ncols, tokens, token_type, scale, logp, lse, entropy, top, top_logp,
                                 top_index, (cudaStream_t)stream);
@@ -532,6 +534,8 @@ int cuvdia_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld
     CUVDIA_REQUIRE(tokens == nullptr || (is_token_type(token_type) && whole_elements(tokens, token_type)));
     CUVDIA_REQUIRE((entropy == nullptr) == (dentropy == nullptr));
     CUVDIA_REQUIRE(dlogp != nullptr || dentropy != nullptr);
+    CUVDIA_REQUIRE(whole_elements(lse, CUVDIA_T_F32) && whole_elements(dlogp, CUVDIA_T_F32));
+    CUVDIA_REQUIRE(whole_elements(entropy, CUVDIA_T_F32) && whole_elements(dentropy, CUVDIA_T_F32));
     if (ncols == 0) return CUVDIA_OK;
     return launch_token_logprob_grad(dlogits, ldd, logits, ld, type, vocab, ncols, tokens, token_type, scale, lse, dlogp,
                                      entropy, dentropy, (cudaStream_t)stream);

@@ -552,7 +552,7 @@ static int logprob_go(const LogprobArgs& q, cudaStream_t st) {
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     if (nvec <= 1024 && q.ncols >= 8 * sm_count()) {
-        cfg.gridDim = dim3((q.ncols + 7) / 8);
+        cfg.gridDim = dim3(((unsigned)q.ncols + 7) / 8);
         CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, TOP, 32>, q, 1));
         return CUVDIA_OK;
     }

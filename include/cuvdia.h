@@ -428,9 +428,10 @@ CUVDIA_API int cuvdia_sequence_f32(float* dst, long long n, void* stream);
  * elements is accepted (columns that start on 16-byte boundaries are the fast case), and rows beyond
  * the row count are neither read nor written.  Element types: CUVDIA_T_F32, CUVDIA_T_F16,
  * CUVDIA_T_BF16; everything is computed in 32 bits and rounded once.  Tokens: CUVDIA_T_I32 or
- * CUVDIA_T_I64; a token outside [0, vocab) - padding - names no token, which is not an error.  Sums
- * are taken in a fixed order (identical bits on every run).  No call allocates; all of them can be
- * recorded into a graph.
+ * CUVDIA_T_I64; a token outside [0, vocab) - padding - names no token, which is not an error.  Row
+ * counts (units, rows, vocab of the logits) go up to 2^30.  Sums are taken in a fixed order (the same
+ * call gives identical bits on every run).  No call allocates; all of them can be recorded into a graph,
+ * on their first call too.
  * ------------------------------------------------------------------------------------------- */
 #define CUVDIA_T_F16  4
 #define CUVDIA_T_BF16 5

@@ -3,15 +3,16 @@ drawn masks, token log probabilities with entropy and alternatives, and their gr
 
 Tolerances count roundings: a result rounded to type t is off by at most eps(t)/2 relative (half the smallest subnormal near
 zero), an operation in 32 bits by 2^-24 relative, the kernels' power of two by 2^-22."""
-import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 import torch
 
 import cuv_b200 as cb
-from cuv_b200 import _capi
 from oracle import host_oracle as ho
 
 pytestmark = pytest.mark.gpu
@@ -555,6 +556,38 @@ def test_on_another_stream_and_in_a_graph():
     torch.cuda.synchronize()
     for (graph, m, b, r), w in zip(made, want):
         assert torch.equal(b["dt"], w[0]) and torch.equal(r.logp, w[1]) and torch.equal(r.top_index, w[2])
+
+
+def test_recorded_on_their_very_first_call():
+    """A process whose first call of every operator is the recorded one."""
+    code = """
+import torch, cuv_b200 as cb
+E = cb.colmajor_empty
+table, x, y, dy, dt = E(96, 300), E(96, 50), E(96, 50), E(96, 50), E(96, 300)
+table.normal_()
+tok, ones = torch.arange(50, device="cuda") % 7, torch.ones(50, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    cb.embedding(x, table, tok)
+    cb.dropout(y, x, 0.5, 1)
+    r = cb.token_logprob(y, tok, entropy=True, top=3)
+    cb.token_logprob_grad(dy, y, r.lse, tok, ones, r.entropy, ones)
+    cb.embedding_grad(dt, tok, dy)
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (x, y, r.lse, r.top_index, dy, dt)]
+cb.embedding(x, table, tok)
+cb.dropout(y, x, 0.5, 1)
+r = cb.token_logprob(y, tok, entropy=True, top=3)
+cb.token_logprob_grad(dy, y, r.lse, tok, ones, r.entropy, ones)
+cb.embedding_grad(dt, tok, dy)
+assert all(torch.equal(a, b) for a, b in zip(got, (x, y, r.lse, r.top_index, dy, dt)))
+assert dt[:, :7].abs().sum() > 0 and (dt[:, 7:] == 0).all()
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "same", run.stderr[-2000:]
 
 
 def test_shapes_types_and_devices_are_refused():

@@ -47,7 +47,7 @@ def test_accepted_without_columns(L):
 
 
 @pytest.mark.parametrize("other", [dict(dst=None), dict(table=None), dict(tokens=None), dict(type=_capi.T_I32), dict(type=I64),
-                                   dict(type=7), dict(token_type=F32), dict(token_type=_capi.T_U8), dict(units=0), dict(vocab=0),
+                                   dict(type=7), dict(token_type=F32), dict(token_type=_capi.T_U8), dict(units=0), dict(vocab=0), dict(units=(1 << 30) + 1, ldd=(1 << 30) + 1, ldt=(1 << 30) + 1),
                                    dict(ncols=-1), dict(ldd=7), dict(ldt=7), dict(dst=ODD), dict(table=ODD), dict(tokens=ODD)])
 def test_embedding_refuses(L, other):
     assert L.cuvdia_embedding(*changed(EMB, **other)) == _capi.ERR_INVALID
@@ -78,6 +78,7 @@ def test_embedding_grad_workspace(L):
 
 
 @pytest.mark.parametrize("other", [dict(dst=None), dict(src=None), dict(draw=None), dict(type=I32), dict(rows=0), dict(ncols=-1),
+                                   dict(rows=(1 << 30) + 1, ldd=(1 << 30) + 1, lds=(1 << 30) + 1),
                                    dict(ldd=7), dict(lds=7), dict(residual=P, ldr=7), dict(p=-0.1), dict(p=1.1),
                                    dict(p=float("nan")), dict(which=-1), dict(which=65536), dict(src=ODD), dict(dst=ODD),
                                    dict(residual=ODD, ldr=8), dict(draw=ctypes.byref(_capi.Draw(1, 1 << 32, 0))),
@@ -89,7 +90,8 @@ def test_dropout_refuses(L, other):
 @pytest.mark.parametrize("other", [dict(logits=None), dict(type=_capi.T_U8), dict(vocab=0), dict(vocab=(1 << 30) + 1, ld=(1 << 30) + 1),
                                    dict(ncols=-1), dict(ld=7), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
                                    dict(scale=float("nan")), dict(tokens=None), dict(logp=None), dict(token_type=F32), dict(top=-1),
-                                   dict(top=33), dict(top_logp=None), dict(top_index=None), dict(logits=ODD), dict(tokens=ODD),
+                                   dict(top=33), dict(top_logp=None), dict(top_index=None), dict(logits=ODD), dict(tokens=ODD), dict(logp=ODD),
+                                   dict(lse=ODD), dict(entropy=ODD), dict(top_logp=ODD), dict(top_index=ODD),
                                    dict(tokens=None, logp=None, lse=None, entropy=None, top=0)])
 def test_token_logprob_refuses(L, other):
     assert L.cuvdia_token_logprob(*changed(LOGP, **other)) == _capi.ERR_INVALID
@@ -98,7 +100,8 @@ def test_token_logprob_refuses(L, other):
 @pytest.mark.parametrize("other", [dict(dlogits=None), dict(logits=None), dict(lse=None), dict(type=I64), dict(vocab=0), dict(ncols=-1),
                                    dict(ld=7), dict(ldd=7), dict(scale=0.0), dict(scale=float("nan")), dict(tokens=None),
                                    dict(dlogp=None), dict(entropy=None), dict(dentropy=None), dict(token_type=F16), dict(dlogits=ODD),
-                                   dict(logits=ODD), dict(tokens=None, dlogp=None, entropy=None, dentropy=None)])
+                                   dict(logits=ODD), dict(lse=ODD), dict(dlogp=ODD), dict(entropy=ODD), dict(dentropy=ODD),
+                                   dict(tokens=None, dlogp=None, entropy=None, dentropy=None)])
 def test_token_logprob_grad_refuses(L, other):
     assert L.cuvdia_token_logprob_grad(*changed(LGRAD, **other)) == _capi.ERR_INVALID
 
