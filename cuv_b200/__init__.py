@@ -543,78 +543,91 @@ def learn_step_weight_decay_momentum(W, momentum, dW, learnrate, momentum_weight
 
 
 # ---- operators of a token model --------------------------------------------------------------------------------
-# These are called once per generated token too, so the checks look at every property once and allocate nothing.
+# These are called once per generated token too, where the checks cost as much as the launch: the usual case is settled in one
+# condition, what is wrong is looked for only when it fails.
 
 _FLOAT_TYPES, _TOKEN_TYPES = {}, {}
+_INT_MAX = 2147483647
 
 
-def _float_type(dtype):
-    """CUVDIA_T_* code of a float type, None for any other."""
-    if not _FLOAT_TYPES:
-        torch = _torch()
-        _TOKEN_TYPES.update({torch.int32: _capi.T_I32, torch.int64: _capi.T_I64})
-        _FLOAT_TYPES.update({torch.float32: _capi.T_F32, torch.float16: _capi.T_F16, torch.bfloat16: _capi.T_BF16})
-    return _FLOAT_TYPES.get(dtype)
+def _fill_types():
+    torch = _torch()
+    _TOKEN_TYPES.update({torch.int32: _capi.T_I32, torch.int64: _capi.T_I64})
+    _FLOAT_TYPES.update({torch.float32: _capi.T_F32, torch.float16: _capi.T_F16, torch.bfloat16: _capi.T_BF16})
 
 
 def _invalid(message):
     raise CuvDiaError(_capi.ERR_INVALID, message)
 
 
-def _matrix(t, name, like=None, shape=None, dtype=None):
-    """(leading dimension, type code) of a column-major matrix in one of the float types; ``like``: a tensor whose device it
-    has to share; ``shape``, ``dtype``: what it has to have."""
+def _matrix(t, name, index=None, code=None, rows=None, cols=None):
+    """(leading dimension, type code, rows, columns, device index) of a column-major CUDA matrix in one of the float types, and
+    with the given device, type and size where these are given."""
+    try:
+        h, w = t.shape
+        between, ld = t.stride()
+        c = _FLOAT_TYPES[t.dtype]
+        dev = t.get_device()
+        if w <= 1:
+            ld = h
+        if ((between == 1 or h == 1) and 0 < h <= ld <= _INT_MAX and w <= _INT_MAX and dev >= 0 and
+                (index is None or dev == index) and (code is None or c == code) and (rows is None or h == rows) and
+                (cols is None or w == cols)):
+            return ld, c, h, w, dev
+    except (AttributeError, KeyError, TypeError, ValueError):
+        pass
+    return _odd_matrix(t, name, index, code, rows, cols)
+
+
+def _odd_matrix(t, name, index, code, rows, cols):
+    if not _FLOAT_TYPES:
+        _fill_types()
+        return _matrix(t, name, index, code, rows, cols)
     if not isinstance(t, _torch().Tensor) or t.dim() != 2:
         _invalid(name + " must be a 2-D tensor")
-    code = _float_type(t.dtype)
-    if code is None:
+    if t.dtype not in _FLOAT_TYPES:
         _invalid(name + " must be a tensor of float32, float16 or bfloat16")
-    if dtype is not None and t.dtype != dtype:
-        _invalid("%s has type %s, not %s" % (name, t.dtype, dtype))
-    rows, cols = t.shape
-    if shape is not None and (rows != shape[0] or cols != shape[1]):
-        _invalid("%s has shape %s, not %s" % (name, (rows, cols), tuple(shape)))
-    between, ld = t.stride()
-    if rows > 1 and between != 1:
+    if code is not None and _FLOAT_TYPES[t.dtype] != code:
+        _invalid("%s has another type than the call's other matrices (%s)" % (name, t.dtype))
+    if rows is not None and t.shape[0] != rows or cols is not None and t.shape[1] != cols:
+        _invalid("%s has shape %s, not (%s, %s)" % (name, tuple(t.shape), "any" if rows is None else rows, "any" if cols is None else cols))
+    if t.shape[0] > 1 and t.stride(0) != 1:
         _invalid(name + " must be column-major (stride(0) == 1)")
-    if cols <= 1:
-        ld = max(rows, 1)
-    if rows < 1 or ld < rows:
+    if t.shape[0] < 1 or t.shape[1] > 1 and t.stride(1) < t.shape[0]:
         _invalid(name + " has no rows or overlapping columns")
-    if ld > 2147483647 or cols > 2147483647:
-        _invalid(name + " has a dimension beyond 2^31 - 1")
-    _on_device(t, name, like)
-    return ld, code
+    if not t.is_cuda:
+        _invalid(name + " must be a CUDA tensor")
+    if index is not None and t.get_device() != index:
+        _invalid("%s is on %s, not on device %d" % (name, t.device, index))
+    _invalid(name + " has a dimension beyond 2^31 - 1")
 
 
-def _vector(t, name, size, like):
-    """A packed float32 vector."""
+def _vector(t, name, size, index):
+    """Address of a packed float32 vector, or None."""
+    if t is None:
+        return None
     if not isinstance(t, _torch().Tensor) or t.dim() != 1 or t.dtype != _torch().float32 or not t.is_contiguous():
         _invalid(name + " must be a contiguous 1-D float32 tensor")
     if t.shape[0] != size:
         _invalid("%s has %d elements, not %d" % (name, t.shape[0], size))
-    _on_device(t, name, like)
+    if t.get_device() != index:
+        _invalid("%s is on %s, not on CUDA device %d" % (name, t.device, index))
+    return t.data_ptr()
 
 
-def _token_type(t, ncols, like):
-    code = _TOKEN_TYPES.get(t.dtype) if isinstance(t, _torch().Tensor) and t.dim() == 1 and t.is_contiguous() else None
-    if code is None:
+def _token_type(t, ncols, index):
+    try:
+        n, = t.shape
+        code = _TOKEN_TYPES[t.dtype]
+        if n == ncols and t.get_device() == index and t.is_contiguous():
+            return code
+    except (AttributeError, KeyError, TypeError, ValueError):
+        pass
+    if not isinstance(t, _torch().Tensor) or t.dim() != 1 or t.dtype not in _TOKEN_TYPES or not t.is_contiguous():
         _invalid("tokens must be a contiguous 1-D int32 or int64 tensor")
     if t.shape[0] != ncols:
         _invalid("tokens has %d elements, not one per column (%d)" % (t.shape[0], ncols))
-    _on_device(t, "tokens", like)
-    return code
-
-
-def _on_device(t, name, like):
-    if not t.is_cuda:
-        _invalid(name + " must be a CUDA tensor")
-    if like is not None and t.get_device() != like.get_device():
-        _invalid("%s is on %s, not on %s" % (name, t.device, like.device))
-
-
-def _address(t):
-    return t.data_ptr() if t is not None else None
+    _invalid("tokens is on %s, not on CUDA device %d" % (t.device, index))
 
 
 def _raw_stream(index):
@@ -624,9 +637,9 @@ def _raw_stream(index):
     return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
-def _call(like, name, *args):
-    """Calls an entry point with the device of the tensor ``like`` current and on its current stream."""
-    cuda, index = _torch().cuda, like.get_device()
+def _call(index, name, *args):
+    """Calls an entry point with device ``index`` current and on its current stream."""
+    cuda = _torch().cuda
     entry = getattr(_capi.lib(), name)
     if cuda.current_device() == index:
         code = entry(*args, _raw_stream(index))
@@ -641,15 +654,11 @@ def embedding(dst, table, tokens, scale=1.0):
     """dst[:, j] = scale * table[:, tokens[j]]; a column of zeros where the token lies outside the table (padding).
     ``table`` is units x vocab, ``dst`` units x ncols, column-major, both float32, float16 or bfloat16; ``tokens`` int32 or
     int64, one per column."""
-    ldt, code = _matrix(table, "table")
-    units, vocab = table.shape
-    ldd, _ = _matrix(dst, "dst", table, None, table.dtype)
-    rows, ncols = dst.shape
-    if rows != units:
-        _invalid("dst has %d rows, the table %d" % (rows, units))
-    tt = _token_type(tokens, ncols, table)
+    ldt, code, units, vocab, index = _matrix(table, "table")
+    ldd, _, _, ncols, _ = _matrix(dst, "dst", index, code, units)
+    tt = _token_type(tokens, ncols, index)
     if ncols:
-        _call(table, "cuvdia_embedding", dst.data_ptr(), ldd, table.data_ptr(), ldt, code, units, vocab, tokens.data_ptr(), tt,
+        _call(index, "cuvdia_embedding", dst.data_ptr(), ldd, table.data_ptr(), ldt, code, units, vocab, tokens.data_ptr(), tt,
               ncols, float(scale))
     return dst
 
@@ -659,20 +668,16 @@ def embedding_grad(dtable, tokens, dout, factNew=1.0, factOld=0.0):
     gradient of :func:`embedding` (``factNew`` = its scale) for the whole table, summed in 32 bits in ascending j.
     ``factOld=0`` writes zeros into the columns of tokens that do not occur; ``factOld=1`` leaves those alone.  ``dtable`` has
     the type of ``dout`` or float32."""
-    torch = _torch()
-    ldo, code = _matrix(dout, "dout")
-    units, ncols = dout.shape
-    ldt, grad_code = _matrix(dtable, "dtable", dout)
-    rows, vocab = dtable.shape
-    if rows != units:
-        _invalid("dtable has %d rows, dout %d" % (rows, units))
+    ldo, code, units, ncols, index = _matrix(dout, "dout")
+    ldt, grad_code, _, vocab, _ = _matrix(dtable, "dtable", index, None, units)
     if grad_code != code and grad_code != _capi.T_F32:
         _invalid("dtable must have dout's type or float32")
-    tt = _token_type(tokens, ncols, dout)
+    tt = _token_type(tokens, ncols, index)
     need = ctypes.c_longlong()
     _capi.check(_capi.lib().cuvdia_embedding_grad_workspace(units, vocab, ncols, ctypes.byref(need)))
+    torch = _torch()
     work = torch.empty(need.value, dtype=torch.uint8, device=dout.device)
-    _call(dout, "cuvdia_embedding_grad", dtable.data_ptr(), ldt, grad_code, dout.data_ptr(), ldo, code, units, vocab,
+    _call(index, "cuvdia_embedding_grad", dtable.data_ptr(), ldt, grad_code, dout.data_ptr(), ldo, code, units, vocab,
           tokens.data_ptr(), tt, ncols, float(factNew), float(factOld), work.data_ptr(), need.value)
     return dtable
 
@@ -681,13 +686,11 @@ def dropout(dst, src, p, seed, step=0, col0=0, which=0, residual=None):
     """dst = (u >= p ? src / (1 - p) : 0) [+ residual], u the uniform number :func:`fill_rnd_uniform` gives for the same
     (seed, step, col0, which): no mask is stored, :func:`dropout_grad` draws the same one again.  float32, float16 or
     bfloat16, all of one type; ``dst`` may be ``src`` or ``residual``."""
-    lds, code = _matrix(src, "src")
-    shape, dtype = src.shape, src.dtype
-    ldd, _ = _matrix(dst, "dst", src, shape, dtype)
-    ldr = _matrix(residual, "residual", src, shape, dtype)[0] if residual is not None else 0
-    rows, ncols = shape
+    lds, code, rows, ncols, index = _matrix(src, "src")
+    ldd = _matrix(dst, "dst", index, code, rows, ncols)[0]
+    ldr, res = (0, None) if residual is None else (_matrix(residual, "residual", index, code, rows, ncols)[0], residual.data_ptr())
     if ncols:
-        _call(src, "cuvdia_dropout", dst.data_ptr(), ldd, src.data_ptr(), lds, _address(residual), ldr, code, rows, ncols, float(p),
+        _call(index, "cuvdia_dropout", dst.data_ptr(), ldd, src.data_ptr(), lds, res, ldr, code, rows, ncols, float(p),
               ctypes.byref(_capi.Draw(int(seed), int(step), int(col0))), int(which))
     return dst
 
@@ -707,26 +710,24 @@ def token_logprob(logits, tokens=None, scale=1.0, entropy=False, top=0):
     and the ``top`` (at most 32) likeliest tokens in descending order, ties to the lowest token: ``top_logp``,
     ``top_index`` of shape (top, ncols).  Returns a :class:`TokenLogprob` of new float32 (int32) tensors, None for what
     was not asked for.  A logit of -inf is a forbidden token."""
-    torch = _torch()
-    ld, code = _matrix(logits, "logits")
-    vocab, ncols = logits.shape
-    tt = _token_type(tokens, ncols, logits) if tokens is not None else 0
+    ld, code, vocab, ncols, index = _matrix(logits, "logits")
+    tt, given = (0, None) if tokens is None else (_token_type(tokens, ncols, index), tokens.data_ptr())
     top = int(top)
     if not 0 <= top <= 32:
         _invalid("0 <= top <= 32")
-    device = logits.device
-    # lse, logp and entropy are rows of one allocation
-    rows = iter(torch.empty((1 + (tokens is not None) + bool(entropy), ncols), dtype=torch.float32, device=device).unbind())
-    lse = next(rows)
-    logp = next(rows) if tokens is not None else None
-    ent = next(rows) if entropy else None
+    torch = _torch()
+    f32, device = torch.float32, logits.device
+    lse = torch.empty(ncols, dtype=f32, device=device)
+    logp = torch.empty_like(lse) if tokens is not None else None
+    ent = torch.empty_like(lse) if entropy else None
     top_logp = top_index = None
     if top:
-        top_logp = torch.empty_strided((top, ncols), (1, top), dtype=torch.float32, device=device)
+        top_logp = torch.empty_strided((top, ncols), (1, top), dtype=f32, device=device)
         top_index = torch.empty_strided((top, ncols), (1, top), dtype=torch.int32, device=device)
     if ncols:
-        _call(logits, "cuvdia_token_logprob", logits.data_ptr(), ld, code, vocab, ncols, _address(tokens), tt, float(scale),
-              _address(logp), lse.data_ptr(), _address(ent), top, _address(top_logp), _address(top_index))
+        _call(index, "cuvdia_token_logprob", logits.data_ptr(), ld, code, vocab, ncols, given, tt, float(scale),
+              None if logp is None else logp.data_ptr(), lse.data_ptr(), None if ent is None else ent.data_ptr(), top,
+              top_logp.data_ptr() if top else None, top_index.data_ptr() if top else None)
     return TokenLogprob(logp, lse, ent, top_logp, top_index)
 
 
@@ -734,15 +735,13 @@ def token_logprob_grad(dlogits, logits, lse, tokens=None, dlogp=None, entropy=No
     """dlogits[v, j] = scale * (dlogp[j]*([v == tokens[j]] - p_v) - dentropy[j]*p_v*(log p_v + entropy[j])): the gradient of a
     loss through :func:`token_logprob`'s ``logp`` (``tokens`` and ``dlogp``) and ``entropy`` (``entropy`` and ``dentropy``);
     ``lse``, ``entropy`` are its results, ``scale`` its scale.  ``dlogits`` has the type of ``logits`` and may be ``logits``."""
-    ld, code = _matrix(logits, "logits")
-    vocab, ncols = logits.shape
-    ldd, _ = _matrix(dlogits, "dlogits", logits, (vocab, ncols), logits.dtype)
-    _vector(lse, "lse", ncols, logits)
-    tt = _token_type(tokens, ncols, logits) if tokens is not None else 0
-    for t, name in ((dlogp, "dlogp"), (entropy, "entropy"), (dentropy, "dentropy")):
-        if t is not None:
-            _vector(t, name, ncols, logits)
+    ld, code, vocab, ncols, index = _matrix(logits, "logits")
+    ldd = _matrix(dlogits, "dlogits", index, code, vocab, ncols)[0]
+    tt, given = (0, None) if tokens is None else (_token_type(tokens, ncols, index), tokens.data_ptr())
+    if lse is None:
+        _invalid("lse is required")
+    vectors = [_vector(t, name, ncols, index) for t, name in ((lse, "lse"), (dlogp, "dlogp"), (entropy, "entropy"), (dentropy, "dentropy"))]
     if ncols:
-        _call(logits, "cuvdia_token_logprob_grad", dlogits.data_ptr(), ldd, logits.data_ptr(), ld, code, vocab, ncols,
-              _address(tokens), tt, float(scale), lse.data_ptr(), _address(dlogp), _address(entropy), _address(dentropy))
+        _call(index, "cuvdia_token_logprob_grad", dlogits.data_ptr(), ldd, logits.data_ptr(), ld, code, vocab, ncols, given, tt,
+              float(scale), *vectors)
     return dlogits
