@@ -18,4 +18,25 @@ __device__ __forceinline__ unsigned in_block(const void* p, unsigned rank) {
     return r;
 }
 
+// Dependent launches: a kernel launched with launch_dependent() may start once every block of the kernel before it in the stream
+// has called launch_dependents() or ended; what it needs from that kernel it may touch after wait_for_dependencies(), which
+// returns when that kernel has ended and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_dependencies() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+inline int launch_dependent(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+    return CUVDIA_OK;
+}
+
 }  // namespace cuvdia

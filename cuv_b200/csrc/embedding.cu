@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(1024, 1)
 sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit_bits, int* __restrict__ keys_out,
                     int* __restrict__ pos_out, int* __restrict__ joins) {
     constexpr int M = 1024 * R;
+    launch_dependents();                                        // whose first blocks need nothing from here
     extern __shared__ unsigned long long pairs[];               // M pairs, then the warps' digit counts, then two rows of digits
     unsigned short (*hist)[SORT_DIGITS] = reinterpret_cast<unsigned short (*)[SORT_DIGITS]>(pairs + M);
     int* total = reinterpret_cast<int*>(hist + 32);
@@ -437,6 +438,7 @@ struct GradOut {
     G* dtable; long long ldt;
     int units, vocab;
     const int* keys; const int* pos; int n;
+    Tokens tokens;
     float* partial; int pitch;                                  // two rows of `pitch` floats a chunk
     int* joins; int chunks;                                     // numbers of short and long joins, then their chunks from both ends
     float fnew, fold;
@@ -454,14 +456,27 @@ __device__ __forceinline__ void finish_column(const GradOut<G>& o, int key, int 
     store_units<T, G, ALIGNED>(to, slice, o.units, acc);
 }
 
-// The columns of 32 tokens that do not occur: zeroed or scaled by a block.
-template <class G>
+// The columns of 32 tokens that do not occur: zeroed or scaled by a block.  Which ones these are it finds in the sorted keys, or,
+// while they are still being sorted (LOOK), by a look through all tokens.
+template <bool LOOK, class G>
 __device__ __forceinline__ void rest_columns(const GradOut<G>& o, long long v0, int* occurs) {
     if (threadIdx.x < 32) {
         const long long v = v0 + threadIdx.x;
-        int lo = 0, hi = o.n;                                   // the first place whose key is not below v
-        while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (o.keys[mid] < v) lo = mid + 1; else hi = mid; }
-        occurs[threadIdx.x] = v >= o.vocab || (lo < o.n && o.keys[lo] == v);
+        bool there = v >= o.vocab;
+        if (!LOOK) {
+            int lo = 0, hi = o.n;                               // the first place whose key is not below v
+            while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (o.keys[mid] < v) lo = mid + 1; else hi = mid; }
+            there = there || (lo < o.n && o.keys[lo] == v);
+        }
+        occurs[threadIdx.x] = there;
+    }
+    if (LOOK) {
+        __syncthreads();
+#pragma unroll 8
+        for (int j = threadIdx.x; j < o.n; j += 256) {
+            const long long t = o.tokens[j] - v0;
+            if (t >= 0 && t < 32) occurs[t] = 1;
+        }
     }
     __syncthreads();
     // a warp a column: a whole block would be half empty on short ones
@@ -486,11 +501,14 @@ __device__ __forceinline__ void rest_columns(const GradOut<G>& o, long long v0, 
 
 template <class T, class G, bool ALIGNED>
 __global__ void __launch_bounds__(256)
-embedding_sum_kernel(const GradOut<G> o, const T* __restrict__ dout, long long ldo, unsigned sum_blocks, int slices) {
+embedding_sum_kernel(const GradOut<G> o, const T* __restrict__ dout, long long ldo, unsigned look_blocks, unsigned sum_blocks,
+                     int slices) {
     constexpr int B = 8;
     __shared__ int occurs[32];
-    if (blockIdx.x >= sum_blocks) { rest_columns(o, (long long)(blockIdx.x - sum_blocks) * 32, occurs); return; }
-    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (blockIdx.x < look_blocks) { rest_columns<true>(o, (long long)blockIdx.x * 32, occurs); return; }
+    wait_for_dependencies();
+    if (blockIdx.x >= look_blocks + sum_blocks) { rest_columns<false>(o, (long long)(blockIdx.x - sum_blocks) * 32, occurs); return; }
+    const long long item = (long long)(blockIdx.x - look_blocks) * 8 + (threadIdx.x >> 5);
     const long long chunk = item / slices;
     const int slice = (int)(item - chunk * slices), lane = threadIdx.x & 31;
     const long long first = chunk * 32;
@@ -541,6 +559,7 @@ template <class G>
 __global__ void __launch_bounds__(256)
 embedding_join_kernel(const GradOut<G> o) {
     __shared__ float4 shares[8][32];
+    wait_for_dependencies();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slices = (o.units + 127) / 128;
     // chunks after this one that begin with the token
     auto followers = [&](int chunk, int key) {
@@ -667,18 +686,24 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     }
     const bool aligned = columns16(dout, ldo, type_size(type)) && columns16(dtable, ldt, type_size(grad_type));
     const long long slices = ((long long)units + 255) / 256, sum_blocks = (g.chunks * slices + 7) / 8;
-    const long long rest_blocks = fold != 1.f ? ((long long)vocab + 31) / 32 : 0;
+    const long long rest_blocks = fold != 1.f ? ((long long)vocab + 31) / 32 : 0, column = (long long)units * type_size(grad_type);
+    // The first columns of absent tokens are written while the tokens are still being sorted, as many as that takes (some 128 MB), by
+    // blocks that look through the tokens themselves where that is little against what they write.  (Only the sort may still be
+    // running then: it is an ordinary launch, so what came before it in the stream has ended.)
+    const long long look_blocks = ncols > 0 && g.cluster && 8LL * ncols <= 64 * column ? std::min(rest_blocks, (128LL << 20) / (32 * column)) : 0;
     if (sum_blocks + rest_blocks > 2147483647LL) { set_last_error("embedding_grad: %lld blocks", sum_blocks + rest_blocks); return CUVDIA_ERR_UNSUPPORTED; }
-    if (sum_blocks + rest_blocks > 0) {
+#define GRAD_OUT(G) {(G*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, toks, (float*)(ws + g.partial), g.pitch, joins, (int)g.chunks, fnew, fold}
 #define SUM_GO(G, A) do {                                                                                                \
-        const GradOut<G> o = {(G*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, joins, (int)g.chunks, fnew, fold}; \
-        embedding_sum_kernel<T, G, A><<<(unsigned)(sum_blocks + rest_blocks), 256, 0, st>>>(o, (const T*)dout, ldo, (unsigned)sum_blocks, (int)slices); \
+        const GradOut<G> o = GRAD_OUT(G);                                                                                \
+        rc = launch_dependent(embedding_sum_kernel<T, G, A>, (unsigned)(sum_blocks + rest_blocks), 256, st, o, (const T*)dout, \
+                              (long long)ldo, (unsigned)look_blocks, (unsigned)sum_blocks, (int)slices);                 \
     } while (0)
+    if (sum_blocks + rest_blocks > 0) {
         CUVDIA_FLOAT_TYPE(type, {
             if (grad_type == type) { if (aligned) SUM_GO(T, true); else SUM_GO(T, false); }
             else { if (aligned) SUM_GO(float, true); else SUM_GO(float, false); }
         });
-#undef SUM_GO
+        if (rc) return rc;
         count_launch();
         rc = check_launch("embedding_sum_kernel");
         if (rc) return rc;
@@ -686,9 +711,12 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     if (g.chunks < 2) return CUVDIA_OK;
     const unsigned join_blocks = (unsigned)std::min((g.chunks - 1) * (((long long)units + 127) / 128), 4LL * sm_count());
     CUVDIA_FLOAT_TYPE(grad_type, {
-        const GradOut<T> o = {(T*)dtable, ldt, units, vocab, keys[src], pos[src], ncols, (float*)(ws + g.partial), g.pitch, joins, (int)g.chunks, fnew, fold};
-        embedding_join_kernel<T><<<join_blocks, 256, 0, st>>>(o);
+        const GradOut<T> o = GRAD_OUT(T);
+        rc = launch_dependent(embedding_join_kernel<T>, join_blocks, 256, st, o);
     });
+#undef SUM_GO
+#undef GRAD_OUT
+    if (rc) return rc;
     count_launch();
     return check_launch("embedding_join_kernel");
 }
