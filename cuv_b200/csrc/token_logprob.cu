@@ -302,53 +302,52 @@ __device__ __forceinline__ void raise(Sums& a, float m, float c) {
     a.m = m;
 }
 
-// Adds a chunk, the U vectors v, v + step, .., to a thread's sums, two elements an instruction.  The sums may be relative to any
-// logit that keeps the powers finite, so the maximum is only looked for in a thread's first chunk (MAX: in every chunk, for
-// callers that want the maximum itself).  A chunk whose sums come out beyond 1e30 or NaN - a logit far above the first chunk's,
-// or an exponent of -inf (a forbidden token) times its power of zero - is summed once more relative to its maximum and with its
-// exponents cut (see LEAST); the others need no test per element.
-template <class T, bool ENT, bool MAX>
-__device__ __forceinline__ void add_chunk(Sums& a, const uint4* v, int step, float c, Where& w, int at) {
+// The sums of a chunk, the U vectors v, v + step, .., relative to the logit m0, two elements an instruction.  CUT: exponents are
+// cut, see LEAST.
+template <class T, bool ENT, bool CUT>
+__device__ __forceinline__ void sum_chunk(const uint4* v, int step, float m0, float c, float2& s, float2& t) {
     constexpr int V = Vec16<T>::N;
-    if (MAX) {
-        const float m = max_chunk<T>(v, step), before = a.m;
-        if (m > before) w.chunk = at;
-        w.second = fmaxf(w.second, fminf(m, before));
-        raise<ENT>(a, m, c);
-    } else if (a.m == -INFINITY) {
-        raise<ENT>(a, max_chunk<T>(v, step), c);
-    }
-    float m0 = shift(a.m);
     const float2 minus = make_float2(-m0, -m0), by = make_float2(c, c);
-    float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
+    s = t = make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float x[V];
         unpack16<T>(v[u * step], x);
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
-            const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), minus), by);
+            float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), minus), by);
             const float2 p = make_float2(exp2_approx(d.x), exp2_approx(d.y));
             s = __fadd2_rn(s, p);
-            if (ENT) t = __ffma2_rn(p, d, t);
-        }
-    }
-    if (!(fabsf(ENT ? t.x + t.y : s.x + s.y) < 1e30f)) {
-        if (!MAX) raise<ENT>(a, max_chunk<T>(v, step), c);
-        m0 = shift(a.m);
-        s = t = make_float2(0.f, 0.f);
-#pragma unroll 1
-        for (int u = 0; u < U; u++) {
-            float x[V];
-            unpack16<T>(v[u * step], x);
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                const float d = (x[e] - m0) * c, p = exp2_approx(d);
-                s.x += p;
-                if (ENT) t.x = fmaf(p, fmaxf(d, LEAST), t.x);
+            if (ENT) {
+                if (CUT) d = make_float2(fmaxf(d.x, LEAST), fmaxf(d.y, LEAST));
+                t = __ffma2_rn(p, d, t);
             }
         }
     }
+}
+
+// Adds a chunk to a thread's sums.  The sums may be relative to any logit that keeps the powers finite, so the maximum is only
+// looked for in a thread's first chunk (MAX: in every chunk, for callers that want the maximum itself).  A chunk whose sums come
+// out beyond 1e30 or NaN - a logit far above the first chunk's, or an exponent of -inf (a forbidden token) times its power of
+// zero - is summed once more, relative to its maximum and with its exponents cut, and so are the thread's later chunks at once
+// (careful); the other threads need no test per element.
+template <class T, bool ENT, bool MAX>
+__device__ __forceinline__ void add_chunk(Sums& a, const uint4* v, int step, float c, Where& w, int at, bool& careful) {
+    if (MAX) {
+        const float m = max_chunk<T>(v, step), before = a.m;
+        if (m > before) w.chunk = at;
+        w.second = fmaxf(w.second, fminf(m, before));
+        raise<ENT>(a, m, c);
+    } else if (a.m == -INFINITY || careful) {
+        raise<ENT>(a, max_chunk<T>(v, step), c);
+    }
+    float2 s, t;
+    if (!careful) {
+        sum_chunk<T, ENT, false>(v, step, shift(a.m), c, s, t);
+        careful = !(fabsf(ENT ? t.x + t.y : s.x + s.y) < 1e30f);
+        if (careful && !MAX) raise<ENT>(a, max_chunk<T>(v, step), c);
+    }
+    if (careful) sum_chunk<T, ENT, ENT>(v, step, shift(a.m), c, s, t);
     a.s = __fadd2_rn(a.s, s);
     if (ENT) a.t = __fadd2_rn(a.t, t);
 }
@@ -418,6 +417,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     const int v0 = (int)((long long)nvec * part / parts), v1 = (int)((long long)nvec * (part + 1) / parts);
     Sums a = {-INFINITY, {0.f, 0.f}, {0.f, 0.f}};
     Where where = {0, -INFINITY};
+    bool careful = false;
     // the given token's logit, fetched here so that it need not be waited for at the end
     bool given = false;
     float given_logit = 0.f;
@@ -450,7 +450,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     for (int k = 0; k < STAGES; k++) fetch(k);
     for (int i = v0; i < v1; i += STEP * U) {
         copies_wait<STAGES - 1>();
-        add_chunk<T, ENT, TOP>(a, mine + stage * (U * THREADS), THREADS, c, where, i + tid - lane);
+        add_chunk<T, ENT, TOP>(a, mine + stage * (U * THREADS), THREADS, c, where, i + tid - lane, careful);
         fetch(stage);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
@@ -556,13 +556,14 @@ static int logprob_go(const LogprobArgs& q, cudaStream_t st) {
         CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, TOP, 32>, q, 1));
         return CUVDIA_OK;
     }
-    // What a call takes, in fifths of the time an SM needs to bring in a chunk of 16 KB: a block's chunks, each at the rate its
-    // SM's blocks leave it but no faster than a round trip to memory allows, and the join of a cluster's blocks (3 us).
+    // What a call takes, in fifths of the time an SM needs to bring in a chunk of 16 KB (0.37 us): a block's chunks, each at the
+    // rate its SM's blocks leave it but no faster than a round trip to memory allows; and for clusters 2 us and 0.7 us a block of
+    // an SM (131072 x 200 bf16 in 1, 2, 4, 8 parts: 16.5, 16.7, 20.5, 22.5 us; 131072 x 4: 14.2 us in one, 8.5 us in 8).
     int parts = 1;
     long long best = 0;
     for (int p = 1; p <= 8; p *= 2) {
         const long long chunks = (nvec + 1024 * p - 1) / (1024 * p), per_sm = ((long long)q.ncols * p + sm_count() - 1) / sm_count();
-        const long long cost = chunks * std::max(5 * per_sm, 6LL) + (p > 1 ? 40 : 0);
+        const long long cost = chunks * std::max(5 * per_sm, 6LL) + (p > 1 ? 27 + 9 * per_sm : 0);
         if (p == 1 || cost < best) { parts = p; best = cost; }
     }
     // Many columns: smaller blocks, of which a thread's share of the joins is smaller.
