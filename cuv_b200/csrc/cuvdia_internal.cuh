@@ -94,7 +94,7 @@ struct cuvdia_plan {
 
 namespace cuvdia {
 // Which uniform numbers a pass draws: key (the seed's two halves), the draw within the step, the step, and the global
-// index of the first batch column the call sees (see glue.cu).
+// index of the first batch column the call sees (see philox.cuh).
 struct DrawParams {
     unsigned k0, k1, which, step;
     long long col0;

@@ -52,10 +52,14 @@ template <class T> struct Streams { T* dst; const T* src; const T* residual; lon
 // vector (SHIFTED = false) a vector's rows are whole groups of the generator.  Where columns start h elements into one (the
 // same h in all matrices), the rows of vector k are E*k - h ..: a lane draws for the rows E*k .. and takes the other h
 // decisions from the lane before it, so nothing is drawn twice but one lane's share of a part.
-// `lanes` threads (a power of two; of one warp if SHIFTED) take a part of a column, U vectors each, `lanes` vectors apart: all loads are in
-// flight before the first number is drawn.  The generator's 32 x 32 bit products keep the heavy multiplier pipe
-// 70 % busy in 16-bit types, where it takes as long as the memory traffic.
-// WIDE: a part is a block's.  NONE: p = 1, every element is dropped.
+// `lanes` threads (a power of two; of one warp if SHIFTED) take a part of a column, U vectors each, `lanes` vectors apart: all
+// loads are in flight before the first number is drawn.  WIDE: a part is a block's.  NONE: p = 1, every element is dropped.
+//
+// Bound by memory where an element is at least six bytes of traffic: 16384 x 8192 bf16 with residual 125 us (6.4 TB/s), 16384 x 4096
+// f32 80 us (6.7 TB/s).  A 16-bit pass without residual (four bytes) is bound by the generator: 17 wide products per four elements
+// keep the multiplier pipe 70 % busy, 115 us at 16384 x 8192 for 82 us of traffic; taking the products' high words from the double
+// units instead gained nothing, the register moves around them costing as much.  Columns that do not start on vectors:
+// 16383 x 8191 with residual 171 us (element by element 315 us).
 template <class T, bool RESIDUAL, bool SHIFTED, bool NONE, int U, bool WIDE>
 __global__ void __launch_bounds__(256, SHIFTED || RESIDUAL ? 4 : 5)
 dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts, const DropoutArgs a) {
@@ -155,14 +159,14 @@ dropout_any_kernel(const Streams<T> m, int rows, int ncols, long long groups, bo
     const T* src = m.src + col * m.lds + i;
     const T* residual = RESIDUAL ? m.residual + col * m.ldr + i : nullptr;
     float x[4], r[4];
-    load_run<T, 4, false>(src, rows - i, x);
-    if (RESIDUAL) load_run<T, 4, false>(residual, rows - i, r);
+    load_run<T, 4>(src, rows - i, x);
+    if (RESIDUAL) load_run<T, 4>(residual, rows - i, r);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const float kept = !none && word[e] >= a.least ? x[e] * a.scale : 0.f;
         x[e] = RESIDUAL ? kept + r[e] : kept;
     }
-    store_run<T, 4, false>(m.dst + col * m.ldd + i, rows - i, x);
+    store_run<T, 4>(m.dst + col * m.ldd + i, rows - i, x);
 }
 
 template <class T, bool RESIDUAL>
@@ -181,7 +185,8 @@ static int dropout_go(const Streams<T>& m, int rows, int ncols, bool none, const
     const bool shifted = !columns16(m.dst, m.ldd, sizeof(T));
     const long long vectors = ((long long)rows + E - 1 + (shifted ? E - 1 : 0)) / E, per = shifted ? 3 : 4;
     // As many lanes a part as leave at most an eighth of a column's parts empty, a whole block at best: its vectors lie
-    // together and its column is known without a division (16384 x 8192 bf16 with residual: 138 us, by warps 150 us).
+    // together and its column is known without a division (16384 x 8192 bf16 with residual: 125 us; parts of a warp each 150 us).
+    // Four vectors a thread (two: 146 us), three where columns are shifted (16383 x 8191: 171 us; two 178, four 195).
     int log_lanes = 0;
     while (log_lanes < 5 && (per << log_lanes) < vectors) log_lanes++;
     if (!shifted)

@@ -108,7 +108,7 @@ int launch_bias_sigmoid_sample(float* act, int ld, const float* bias, const floa
 // reproducible run to run.  Summed is either the activation after the logistic or the 0/1 sample; this replaces a
 // separate reduce_to_col over a matrix this pass has just produced.  With store_act == 0 the activations are
 // not written back (callers that only consume the sample and its sum).
-// DRAW: the uniform numbers are not read from u but drawn in registers (see draw4 above).
+// DRAW: the uniform numbers are not read from u but drawn in registers (see draw4 in philox.cuh).
 template <bool VEC, bool DRAW>
 __global__ void __launch_bounds__(256)
 bias_sigmoid_sample_sum_kernel(float* __restrict__ act, int ld, const float* __restrict__ bias,

@@ -72,41 +72,17 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int PENDING>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
-// N consecutive elements at p: one 128-bit access per 16 bytes (p 16-byte aligned), or, where ALIGNED is false or the
-// range ends inside, element by element up to `n` of them.
-template <class T, int N, bool ALIGNED>
-__device__ __forceinline__ void load_run(const T* __restrict__ p, int n, float (&x)[N]) {
-    constexpr int V = Vec16<T>::N;
-    static_assert(!ALIGNED || N % V == 0, "whole vectors");
-    if (ALIGNED && n >= N) {
+// up to N consecutive elements at p, element by element: the first n of them, zero for the rest
+template <class T, int N>
+__device__ __forceinline__ void load_run(const T* p, int n, float (&x)[N]) {
 #pragma unroll
-        for (int q = 0; q < N / V; q++) {
-            float y[V];
-            unpack16<T>(*reinterpret_cast<const uint4*>(p + q * V), y);
-#pragma unroll
-            for (int e = 0; e < V; e++) x[q * V + e] = y[e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; e++) x[e] = e < n ? to_f32(p[e]) : 0.f;
-    }
+    for (int e = 0; e < N; e++) x[e] = e < n ? to_f32(p[e]) : 0.f;
 }
 
-template <class T, int N, bool ALIGNED>
-__device__ __forceinline__ void store_run(T* __restrict__ p, int n, const float (&x)[N]) {
-    constexpr int V = Vec16<T>::N;
-    if (ALIGNED && n >= N) {
+template <class T, int N>
+__device__ __forceinline__ void store_run(T* p, int n, const float (&x)[N]) {
 #pragma unroll
-        for (int q = 0; q < N / V; q++) {
-            float y[V];
-#pragma unroll
-            for (int e = 0; e < V; e++) y[e] = x[q * V + e];
-            *reinterpret_cast<uint4*>(p + q * V) = pack16<T>(y);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; e++) if (e < n) p[e] = from_f32<T>(x[e]);
-    }
+    for (int e = 0; e < N; e++) if (e < n) p[e] = from_f32<T>(x[e]);
 }
 
 // The 16 bytes that begin `bytes` (0 .. 15, whole elements) behind the start of a, where b follows a in memory.
