@@ -508,7 +508,7 @@ int cuvdia_token_logprob(const void* logits, int ld, int type, int vocab, int nc
     CUVDIA_REQUIRE(whole_elements(logits, type));
     CUVDIA_REQUIRE(vocab > 0 && vocab <= (1 << 30) && ncols >= 0);
     CUVDIA_REQUIRE(ld >= vocab);
-    CUVDIA_REQUIRE(scale > 0.f && scale <= 3.402823466e38f);
+    CUVDIA_REQUIRE(scale > 0.f && scale <= 1e30f);
     CUVDIA_REQUIRE((tokens == nullptr) == (logp == nullptr));
     CUVDIA_REQUIRE(tokens == nullptr || (is_token_type(token_type) && whole_elements(tokens, token_type)));
     CUVDIA_REQUIRE(top >= 0 && top <= 32);
@@ -529,7 +529,7 @@ int cuvdia_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld
     CUVDIA_REQUIRE(whole_elements(dlogits, type) && whole_elements(logits, type));
     CUVDIA_REQUIRE(vocab > 0 && vocab <= (1 << 30) && ncols >= 0);
     CUVDIA_REQUIRE(ld >= vocab && ldd >= vocab);
-    CUVDIA_REQUIRE(scale > 0.f && scale <= 3.402823466e38f);
+    CUVDIA_REQUIRE(scale > 0.f && scale <= 1e30f);
     CUVDIA_REQUIRE((tokens == nullptr) == (dlogp == nullptr));
     CUVDIA_REQUIRE(tokens == nullptr || (is_token_type(token_type) && whole_elements(tokens, token_type)));
     CUVDIA_REQUIRE((entropy == nullptr) == (dentropy == nullptr));

@@ -472,7 +472,7 @@ CUVDIA_API int cuvdia_dropout(void* dst, int ldd, const void* src, int lds, cons
  * Any of lse, logp (with tokens) and entropy may be NULL, not all with top == 0; 0 <= top <= 32.  A logit of -inf is
  * a forbidden token: probability zero, never among the likeliest; places left over hold index -1 and -inf.
  * A column without any finite logit gives lse = logp = -inf, entropy 0.  A NaN or +inf logit makes lse, logp and
- * entropy NaN (NaN is never among the likeliest).  scale is finite and positive. */
+ * entropy NaN (NaN is never among the likeliest).  0 < scale <= 1e30. */
 CUVDIA_API int cuvdia_token_logprob(const void* logits, int ld, int type, int vocab, int ncols, const void* tokens,
                                     int token_type, float scale, float* logp, float* lse, float* entropy, int top,
                                     float* top_logp, int* top_index, void* stream);

@@ -88,7 +88,7 @@ def test_dropout_refuses(L, other):
 
 
 @pytest.mark.parametrize("other", [dict(logits=None), dict(type=_capi.T_U8), dict(vocab=0), dict(vocab=(1 << 30) + 1, ld=(1 << 30) + 1),
-                                   dict(ncols=-1), dict(ld=7), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
+                                   dict(ncols=-1), dict(ld=7), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=2e30),
                                    dict(scale=float("nan")), dict(tokens=None), dict(logp=None), dict(token_type=F32), dict(top=-1),
                                    dict(top=33), dict(top_logp=None), dict(top_index=None), dict(logits=ODD), dict(tokens=ODD), dict(logp=ODD),
                                    dict(lse=ODD), dict(entropy=ODD), dict(top_logp=ODD), dict(top_index=ODD),
@@ -139,3 +139,28 @@ def test_python_refuses(call, says):
     with pytest.raises(cb.CuvDiaError) as e:
         call()
     assert e.value.code == _capi.ERR_INVALID and says in str(e.value)
+
+
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    """With another device current, a call enters the tensors' device and takes that device's stream."""
+    import contextlib
+    seen = []
+
+    @contextlib.contextmanager
+    def device(index):
+        seen.append(("enter", index))
+        yield
+        seen.append(("leave", index))
+
+    class Lib:
+        def entry(self, *args):
+            seen.append(args)
+            return 0
+
+    monkeypatch.setattr(_capi, "lib", lambda: Lib())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(cb, "_raw_stream", lambda index: 1000 + index)
+    cb._call(0, "entry", 7)
+    cb._call(2, "entry", 8)
+    assert seen == [(7, 1000), ("enter", 2), (8, 1002), ("leave", 2)]
