@@ -475,7 +475,8 @@ int cuvdia_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     CUVDIA_REQUIRE(ldt >= units);
     CUVDIA_REQUIRE(whole_elements(dtable, grad_type));
     if (ncols > 0) {
-        CUVDIA_REQUIRE(dout != nullptr && tokens != nullptr && workspace != nullptr);
+        CUVDIA_REQUIRE(dout != nullptr && tokens != nullptr);
+        CUVDIA_REQUIRE(workspace != nullptr || embedding_grad_bytes(units, vocab, ncols) == 0);
         CUVDIA_REQUIRE(ldo >= units);
         CUVDIA_REQUIRE(whole_elements(dout, type) && whole_elements(tokens, token_type));
         CUVDIA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0);

@@ -447,8 +447,9 @@ CUVDIA_API int cuvdia_embedding(void* dst, int ldd, const void* table, int ldt, 
  * dtable is not read, columns of tokens that do not occur become zero.  factOld == 1: only columns of
  * tokens that occur are touched (gradients accumulated over several batches).  grad_type is `type`
  * (dout's) or CUVDIA_T_F32.  The positions are sorted by token inside the call; `workspace` is device
- * memory of cuvdia_embedding_grad_workspace(units, vocab, ncols) bytes at least, 16-byte aligned, its
- * contents undefined before and after; two calls that may overlap need two.  ncols <= 2^30. */
+ * memory of cuvdia_embedding_grad_workspace(units, vocab, ncols) bytes at least (0 for few positions: it may
+ * be NULL then), 16-byte aligned, its contents undefined before and after; two calls that may overlap need two.
+ * ncols <= 2^30. */
 CUVDIA_API int cuvdia_embedding_grad_workspace(int units, int vocab, int ncols, long long* bytes);
 CUVDIA_API int cuvdia_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout, int ldo, int type, int units,
                                      int vocab, const void* tokens, int token_type, int ncols, float factNew,

@@ -131,7 +131,7 @@ def test_embedding_grad(kind, grad, units, ld, offset, vocab, ncols):
         outside_untouched(buf, dtable)
 
 
-@pytest.mark.parametrize("ncols", [31, 1024, 1025, 4095, 4097, 8192, 8193, 16384, 20000, 32769, 70001, 131072, 131073, 300001])
+@pytest.mark.parametrize("ncols", [31, 256, 257, 1024, 1025, 4095, 4097, 8192, 8193, 16384, 20000, 32769, 70001, 131072, 131073, 300001])
 @pytest.mark.parametrize("vocab", [2, 511, 512, 131071, 300007])
 def test_embedding_grad_sums_whole_numbers_exactly(ncols, vocab):
     """Whole numbers whose sums stay below 2^24: equality, whatever the order; text-like frequencies, so that single
@@ -149,8 +149,9 @@ def test_embedding_grad_sums_whole_numbers_exactly(ncols, vocab):
 
 
 @pytest.mark.parametrize("case", ["one token", "all padding", "no columns", "ascending", "descending"])
-def test_embedding_grad_extremes(case):
-    units, vocab, ncols = 40, 3000, 0 if case == "no columns" else 2500
+@pytest.mark.parametrize("many", [200, 2500])
+def test_embedding_grad_extremes(case, many):
+    units, vocab, ncols = 40, 3000, 0 if case == "no columns" else many
     dout = torch.randint(-9, 10, (ncols, units), device="cuda", generator=gen(1)).float().t()
     tok = {"one token": torch.full((ncols,), 17), "all padding": torch.full((ncols,), -1), "no columns": torch.empty(0, dtype=torch.long),
            "ascending": torch.arange(ncols), "descending": vocab - 1 - torch.arange(ncols)}[case].cuda()

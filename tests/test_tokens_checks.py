@@ -29,7 +29,7 @@ def changed(good, **other):
 
 
 EMB = dict(dst=P, ldd=8, table=P, ldt=8, type=BF16, units=8, vocab=5, tokens=P, token_type=I64, ncols=0, scale=1.0, stream=None)
-GRAD = dict(dtable=P, ldt=8, grad_type=F32, dout=P, ldo=8, type=BF16, units=8, vocab=5, tokens=P, token_type=I32, ncols=3,
+GRAD = dict(dtable=P, ldt=8, grad_type=F32, dout=P, ldo=8, type=BF16, units=8, vocab=5, tokens=P, token_type=I32, ncols=5000,
             fnew=1.0, fold=0.0, work=P, bytes=1 << 30, stream=None)
 DROP = dict(dst=P, ldd=8, src=P, lds=8, residual=None, ldr=0, type=F16, rows=8, ncols=0, p=0.5, draw=ctypes.byref(DRAW), which=0,
             stream=None)
@@ -68,8 +68,9 @@ def test_embedding_grad_workspace(L):
         assert L.cuvdia_embedding_grad_workspace(*bad, ctypes.byref(n)) == _capi.ERR_INVALID
     assert L.cuvdia_embedding_grad_workspace(8, 5, 3, None) == _capi.ERR_INVALID
     assert L.cuvdia_embedding_grad_workspace(8, 5, 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert L.cuvdia_embedding_grad_workspace(4096, 131072, 8, ctypes.byref(n)) == 0 and n.value == 0       # few: none
     last = 0
-    for ncols in (1, 1000, 100000, 1 << 24, 1 << 30):
+    for ncols in (5000, 100000, 1 << 24, 1 << 30):
         assert L.cuvdia_embedding_grad_workspace(4096, 131072, ncols, ctypes.byref(n)) == 0
         assert n.value > last
         last = n.value
