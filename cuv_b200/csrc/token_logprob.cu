@@ -612,22 +612,26 @@ int launch_token_logprob(const void* logits, int ld, int type, int vocab, int nc
 //   dlogits_v = 2^(d log2 e) * (A d + B) (+ scale * dlogp at the token),   A = -scale dentropy,  B = -scale (dlogp + dentropy entropy)
 // two elements an instruction.  A block owns up to 1024 vectors of one column, those of the logits' memory; the stores are vectors
 // too where dlogits lies alike, else element by element.  In place is fine: a thread reads its elements before it writes them.
-// Bound by memory: 32768 x 8192 bf16 168 us, with entropies 176 us (6.1 TB/s); 32768 x 4096 f32 173 us.
+// Bound by memory: 32768 x 8192 bf16 with or without entropies 158 us (6.8 TB/s), 32768 x 4096 f32 160 us.  The straight-line path
+// for blocks that lie inside a column is what that took (one path with tests per vector: 176 us).
 struct GradFactors { float scale, minus_lse, a, b; };
 
-// a vector's gradients but for the token's own term; CUT: exponents are cut, see LEAST
+// two gradients but for the token's own term; CUT: exponents are cut, see LEAST
+template <bool ENT, bool CUT>
+__device__ __forceinline__ void grad_pair(float& x, float& y, const GradFactors& f) {
+    float2 d = __ffma2_rn(make_float2(x, y), make_float2(f.scale, f.scale), make_float2(f.minus_lse, f.minus_lse));
+    const float2 q = __fmul2_rn(d, make_float2(LOG2E, LOG2E));
+    const float2 p = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+    if (ENT && CUT) d = make_float2(fmaxf(d.x, LEAST), fmaxf(d.y, LEAST));
+    const float2 b = make_float2(f.b, f.b);
+    const float2 r = __fmul2_rn(p, ENT ? __ffma2_rn(d, make_float2(f.a, f.a), b) : b);
+    x = r.x; y = r.y;
+}
+
 template <class T, bool ENT, bool CUT>
 __device__ __forceinline__ void grad_vector(float (&x)[Vec16<T>::N], const GradFactors& f) {
 #pragma unroll
-    for (int e = 0; e < Vec16<T>::N; e += 2) {
-        float2 d = __ffma2_rn(make_float2(x[e], x[e + 1]), make_float2(f.scale, f.scale), make_float2(f.minus_lse, f.minus_lse));
-        const float2 q = __fmul2_rn(d, make_float2(LOG2E, LOG2E));
-        const float2 p = make_float2(exp2_approx(q.x), exp2_approx(q.y));
-        if (ENT && CUT) d = make_float2(fmaxf(d.x, LEAST), fmaxf(d.y, LEAST));
-        const float2 b = make_float2(f.b, f.b);
-        const float2 r = __fmul2_rn(p, ENT ? __ffma2_rn(d, make_float2(f.a, f.a), b) : b);
-        x[e] = r.x; x[e + 1] = r.y;
-    }
+    for (int e = 0; e < Vec16<T>::N; e += 2) grad_pair<ENT, CUT>(x[e], x[e + 1], f);
 }
 
 template <class T, bool ENT, int THREADS>
@@ -640,7 +644,9 @@ token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long 
     const int chunk = blockIdx.x - (unsigned)col * (unsigned)chunks;
     const T* x0 = logits + col * ld;
     T* y0 = dlogits + col * ldd;
-    const int head = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));      // elements before x0 in its first vector
+    // whole vectors of the column, behind `head` elements and before the rest
+    const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)));
+    const int nvec = (vocab - head) / V, rest = vocab - head - nvec * V;
     const bool alike = ((reinterpret_cast<uintptr_t>(x0) ^ reinterpret_cast<uintptr_t>(y0)) & 15) == 0;
     const float l = lse[col];
     long long t = dlogp ? tokens[col] : -1;
@@ -648,46 +654,50 @@ token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long 
     // A padded column without an entropy term is zero without a look at its logits, and so is a column that has no
     // finite logit.
     const bool zero = (t < 0 && !ENT) || l == -INFINITY;
-    const int first = (chunk * (THREADS * U) + (int)threadIdx.x) * V - head;
+    const uint4* from = reinterpret_cast<const uint4*>(x0 + head);
+    T* to = y0 + head;
+    const int v0 = chunk * (THREADS * U) + (int)threadIdx.x;
+    const bool plain = alike && !zero && (chunk + 1) * (THREADS * U) <= nvec;           // as most blocks are
     uint4 raw[U];
+    if (plain) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int e0 = first + u * (THREADS * V);
-        if (!zero && e0 >= 0 && e0 + V <= vocab) raw[u] = *reinterpret_cast<const uint4*>(x0 + e0);
+        for (int u = 0; u < U; u++) raw[u] = from[v0 + u * THREADS];
     }
     const float g = t >= 0 ? dlogp[col] : 0.f, h = ENT ? dentropy[col] : 0.f, hot = scale * g;
     const GradFactors f = {scale, -l, -scale * h, -scale * (ENT ? fmaf(h, entropy[col], g) : g)};
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int e0 = first + u * (THREADS * V);
-        if (e0 >= vocab) break;
-        const bool whole = e0 >= 0 && e0 + V <= vocab;
+    const int token = t >= 0 ? (int)t - head : -1;              // the token's place behind the whole vectors' start
+    // a whole vector's gradients; 0 * -inf comes up only where the least exponent is out of all proportion (a forbidden token)
+    auto whole_vector = [&](const uint4& r, int v) {
         float x[V];
-        if (zero) {
+        unpack16<T>(r, x);
+        if (ENT && fmaf(min_raw(r, T()), scale, -l) < LEAST) grad_vector<T, ENT, true>(x, f);
+        else grad_vector<T, ENT, false>(x, f);
+        const unsigned at = (unsigned)(token - v * V);
+        if (at < V && token >= 0) {
 #pragma unroll
-            for (int e = 0; e < V; e++) x[e] = 0.f;
-        } else {
-            if (whole) {
-                unpack16<T>(raw[u], x);
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; e++) x[e] = e0 + e >= 0 && e0 + e < vocab ? to_f32(x0[e0 + e]) : 0.f;
-            }
-            // 0 * -inf comes up only where the least exponent is out of all proportion (a forbidden token)
-            if (ENT && (!whole || fmaf(min_raw(raw[u], T()), scale, -l) < LEAST)) grad_vector<T, ENT, true>(x, f);
-            else grad_vector<T, ENT, false>(x, f);
-            const unsigned at = (unsigned)((int)t - e0);
-            if (at < V && t >= 0) {
-#pragma unroll
-                for (int e = 0; e < V; e++) if (e == (int)at) x[e] += hot;
-            }
+            for (int e = 0; e < V; e++) if (e == (int)at) x[e] += hot;
         }
-        if (alike && whole) {
-            *reinterpret_cast<uint4*>(y0 + e0) = pack16<T>(x);
-        } else {
+        return pack16<T>(x);
+    };
+    if (plain) {
 #pragma unroll
-            for (int e = 0; e < V; e++) if (e0 + e >= 0 && e0 + e < vocab) y0[e0 + e] = from_f32<T>(x[e]);
+        for (int u = 0; u < U; u++) reinterpret_cast<uint4*>(to)[v0 + u * THREADS] = whole_vector(raw[u], v0 + u * THREADS);
+    } else {
+#pragma unroll 1
+        for (int v = v0; v < min(nvec, (chunk + 1) * (THREADS * U)); v += THREADS) {
+            const uint4 r = zero ? make_uint4(0, 0, 0, 0) : whole_vector(from[v], v);
+            if (alike) { reinterpret_cast<uint4*>(to)[v] = r; continue; }
+            float x[V];
+            unpack16<T>(r, x);
+#pragma unroll
+            for (int e = 0; e < V; e++) to[v * V + e] = from_f32<T>(x[e]);
         }
+    }
+    if (chunk == 0 && (int)threadIdx.x < head + rest) {         // the ends, one element a thread
+        const int i = (int)threadIdx.x < head ? (int)threadIdx.x : nvec * V + (int)threadIdx.x;
+        float x[2] = {zero ? 0.f : to_f32(x0[i]), 0.f};
+        if (!zero) grad_pair<ENT, true>(x[0], x[1], f);
+        y0[i] = from_f32<T>(zero ? 0.f : t == i ? x[0] + hot : x[0]);
     }
 }
 
@@ -697,7 +707,7 @@ int launch_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld
     const int v = 16 / type_size(type);
     // blocks of 1024 vectors, of 256 where a column has no more (1000 x 4000 bf16: 8.2 us, with large blocks 12.3 us)
     const int threads = vocab > 256 * v ? 256 : 64;
-    const long long per = threads * U * v, chunks = ((long long)vocab + v - 1 + per - 1) / per;       // up to v - 1 elements of offset
+    const long long chunks = std::max(1LL, ((long long)vocab / v + threads * U - 1) / (threads * U));
     const long long blocks = chunks * ncols;
     if (blocks > 2147483647LL) { set_last_error("token_logprob_grad: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
 #define LG_GO(E, N) token_logprob_grad_kernel<T, E, N><<<(unsigned)blocks, N, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld, \
