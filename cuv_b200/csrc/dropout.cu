@@ -83,24 +83,13 @@ dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts
     T* d = m.dst + col * m.ldd;
     const int h = SHIFTED ? (int)((reinterpret_cast<uintptr_t>(d) & 15) / sizeof(T)) : 0;
     const int w0 = part * span + l, i0 = w0 * E - h;
-    uint4 xs[U], rs[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int i = i0 + u * lanes * E;
-        if (!idle && (!SHIFTED || i >= 0) && i + E <= rows) {
-            xs[u] = *reinterpret_cast<const uint4*>(s + i);
-            if (RESIDUAL) rs[u] = *reinterpret_cast<const uint4*>(r + i);
-        }
-    }
     const long long gcol = a.col0 + col;
     unsigned long long first = (unsigned long long)M0 * (unsigned)(w0 * (E / 4));
     const unsigned long long first_step = (unsigned long long)M0 * (unsigned)(lanes * (E / 4));
     unsigned before = 0;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int i = i0 + u * lanes * E;
-        if (!SHIFTED && i >= rows) break;
-        unsigned word[E], mask = 0;
+    // the decisions for vector u, which comes after u - 1: words, or (SHIFTED) bits
+    auto decide = [&](int u, unsigned (&word)[E]) {
+        unsigned mask = 0;
         if (!NONE) draw<E>(a, first, gcol, word);
         first += first_step;
         if (SHIFTED) {
@@ -113,21 +102,10 @@ dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts
             if (u > 0 && l == 0) prev = last;
             before = mask;
             mask = (prev | mask << E) >> (E - h);
-            if (idle || i >= rows || (part > 0 && u == 0 && l == 0)) continue;         // that lane only drew for the next one
         }
-        const bool whole = (!SHIFTED || i >= 0) && i + E <= rows;
-        float x[E], y[E];
-        if (whole) {
-            unpack16<T>(xs[u], x);
-            if (RESIDUAL) unpack16<T>(rs[u], y);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool in = i + e >= 0 && i + e < rows;
-                x[e] = in ? to_f32(s[i + e]) : 0.f;
-                if (RESIDUAL) y[e] = in ? to_f32(r[i + e]) : 0.f;
-            }
-        }
+        return mask;
+    };
+    auto apply = [&](float (&x)[E], const float (&y)[E], const unsigned (&word)[E], unsigned mask) {
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             const float2 scaled = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(a.scale, a.scale));
@@ -137,6 +115,54 @@ dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts
             const float2 sum = RESIDUAL ? __fadd2_rn(kept, make_float2(y[e], y[e + 1])) : kept;
             x[e] = sum.x; x[e + 1] = sum.y;
         }
+    };
+    const bool ghost = SHIFTED && part > 0 && l == 0;           // whose first vector is the lane's before: drawn, not written
+    // threads whose vectors all lie inside the column, as most do, take a straight line; shifted columns have ends enough to be
+    // left to one path, which loads ahead too
+    const bool plain = !SHIFTED && i0 + ((U - 1) * lanes + 1) * E <= rows;
+    uint4 xs[U], ys[U];
+    if (plain || SHIFTED) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * lanes * E;
+            if (SHIFTED && (idle || i < 0 || i + E > rows)) continue;
+            xs[u] = *reinterpret_cast<const uint4*>(s + i);
+            if (RESIDUAL) ys[u] = *reinterpret_cast<const uint4*>(r + i);
+        }
+    }
+    if (plain) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            unsigned word[E];
+            const unsigned mask = decide(u, word);
+            float x[E], y[E];
+            unpack16<T>(xs[u], x);
+            if (RESIDUAL) unpack16<T>(ys[u], y);
+            apply(x, y, word, mask);
+            *reinterpret_cast<uint4*>(d + i0 + u * lanes * E) = pack16<T>(x);
+        }
+        return;
+    }
+#pragma unroll (SHIFTED ? U : 1)
+    for (int u = 0; u < U; u++) {
+        const int i = i0 + u * lanes * E;
+        unsigned word[E];
+        const unsigned mask = decide(u, word);
+        if (idle || i >= rows || (u == 0 && ghost)) continue;
+        const bool whole = i >= 0 && i + E <= rows;
+        float x[E], y[E];
+        if (whole) {
+            unpack16<T>(SHIFTED ? xs[u] : *reinterpret_cast<const uint4*>(s + i), x);
+            if (RESIDUAL) unpack16<T>(SHIFTED ? ys[u] : *reinterpret_cast<const uint4*>(r + i), y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const bool in = i + e >= 0 && i + e < rows;
+                x[e] = in ? to_f32(s[i + e]) : 0.f;
+                if (RESIDUAL) y[e] = in ? to_f32(r[i + e]) : 0.f;
+            }
+        }
+        apply(x, y, word, mask);
         if (whole) {
             *reinterpret_cast<uint4*>(d + i) = pack16<T>(x);
         } else {
