@@ -55,13 +55,13 @@ template <class T> struct Streams { T* dst; const T* src; const T* residual; lon
 // `lanes` threads (a power of two; of one warp if SHIFTED) take a part of a column, U vectors each, `lanes` vectors apart: all
 // loads are in flight before the first number is drawn.  WIDE: a part is a block's.  NONE: p = 1, every element is dropped.
 //
-// Bound by memory where an element is at least six bytes of traffic: 16384 x 8192 bf16 with residual 125 us (6.4 TB/s), 16384 x 4096
-// f32 80 us (6.7 TB/s).  A 16-bit pass without residual (four bytes) is bound by the generator: 17 wide products per four elements
-// keep the multiplier pipe 70 % busy, 115 us at 16384 x 8192 for 82 us of traffic; taking the products' high words from the double
+// Bound by memory where an element is at least six bytes of traffic: 16384 x 8192 bf16 with residual 117 us (6.9 TB/s), 16384 x 4096
+// f32 80 us (6.7 TB/s).  A 16-bit pass without residual (four bytes) is bound by the generator, whose 17 wide products per four
+// elements fill the multiplier pipe: 107 us at 16384 x 8192 for 82 us of traffic; taking the products' high words from the double
 // units instead gained nothing, the register moves around them costing as much.  Columns that do not start on vectors:
-// 16383 x 8191 with residual 171 us (element by element 315 us).
+// 16383 x 8191 with residual 172 us (element by element 315 us).
 template <class T, bool RESIDUAL, bool SHIFTED, bool NONE, int U, bool WIDE>
-__global__ void __launch_bounds__(256, SHIFTED || RESIDUAL ? 4 : 5)
+__global__ void __launch_bounds__(256, 4)
 dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts, const DropoutArgs a) {
     constexpr int E = Vec16<T>::N;
     const int lanes = WIDE ? 256 : 1 << log_lanes, l = threadIdx.x & (lanes - 1), span = lanes * U - (SHIFTED ? 1 : 0);
@@ -211,8 +211,9 @@ static int dropout_go(const Streams<T>& m, int rows, int ncols, bool none, const
     const bool shifted = !columns16(m.dst, m.ldd, sizeof(T));
     const long long vectors = ((long long)rows + E - 1 + (shifted ? E - 1 : 0)) / E, per = shifted ? 3 : 4;
     // As many lanes a part as leave at most an eighth of a column's parts empty, a whole block at best: its vectors lie
-    // together and its column is known without a division (16384 x 8192 bf16 with residual: 125 us; parts of a warp each 150 us).
-    // Four vectors a thread (two: 146 us), three where columns are shifted (16383 x 8191: 171 us; two 178, four 195).
+    // together and its column is known without a division (16384 x 8192 bf16 with residual: 125 us when this was
+    // chosen, parts of a warp each 150 us).  Four vectors a thread (two: 146 us), three where columns are shifted (16383 x 8191:
+    // 171 us; two 178, four 195).
     int log_lanes = 0;
     while (log_lanes < 5 && (per << log_lanes) < vectors) log_lanes++;
     if (!shifted)
