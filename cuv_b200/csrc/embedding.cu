@@ -142,7 +142,7 @@ __device__ __forceinline__ unsigned same_digit(int digit, int bits) {
 template <int R>
 __global__ void __launch_bounds__(1024, 1)
 sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit_bits, int* __restrict__ keys_out,
-                    int* __restrict__ pos_out, int* __restrict__ joins) {
+                    int* __restrict__ pos_out, int4* __restrict__ joins) {
     constexpr int M = 1024 * R;
     launch_dependents();                                        // whose first blocks need nothing from here
     extern __shared__ unsigned long long pairs[];               // M pairs, then the warps' digit counts, then two rows of digits
@@ -155,7 +155,7 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << digit_bits;
     const int g0 = (int)rank_in * M + warp * (32 * R) + lane;
-    if (rank_in == 0 && threadIdx.x < 2) joins[threadIdx.x] = 0;
+    if (rank_in == 0 && threadIdx.x == 0) joins[0] = make_int4(0, 0, 0, 0);
     int key[R], pos[R], place[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -236,7 +236,7 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
 
 template <int R>
 static int sort_cluster(int blocks, const Tokens& tokens, int n, int vocab, int passes, int digit_bits, int* keys, int* pos,
-                        int* joins, cudaStream_t st) {
+                        int4* joins, cudaStream_t st) {
     static bool done[64] = {false};
     const size_t bytes = 1024 * R * 8 + 32 * SORT_DIGITS * 2 + 2 * SORT_DIGITS * 4;
     int rc = allow_dynamic_smem(sort_cluster_kernel<R>, bytes, done);
@@ -284,9 +284,9 @@ sort_count_kernel(const Tokens tokens, const int* __restrict__ keys, int n, int 
 }
 
 // exclusive scan of `n` counts in place, one block
-__global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ counts, long long n, int* __restrict__ joins) {
+__global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ counts, long long n, int4* __restrict__ joins) {
     __shared__ int warp_sum[32];
-    if (threadIdx.x < 2) joins[threadIdx.x] = 0;
+    if (threadIdx.x == 0) joins[0] = make_int4(0, 0, 0, 0);
     const long long per = (n + 1023) / 1024, first = per * threadIdx.x, last = min(n, first + per);
     int sum = 0;
     for (long long k = first; k < last; k++) sum += counts[k];
@@ -360,8 +360,8 @@ sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* _
 // border leaves a partial sum: slot 0 of the chunk if the token began in an earlier one, else slot 1; the second kernel adds a
 // token's partial sums, in the order of the chunks or of a fixed split of them.  Behind the blocks that sum come those that
 // write the columns of tokens that do not occur, 32 columns each: stores that fill the memory's time between the loads.
-// Bound by memory but for the sort and the joins, 12 us each: 4096 x 32768 f32 from 16384 bf16 columns 132 us (103 us of
-// traffic), 1024 x 131072 from 8192 bf16 59 us (44 us).  Longer chunks leave fewer partial sums but too few warps: with blocks
+// Bound by memory but for the joins and what the sums' launch does not hide of the sort: 4096 x 32768 f32 from 16384 bf16 columns
+// 129 us (103 us of traffic), 1024 x 131072 from 8192 bf16 57 us (44 us).  Longer chunks leave fewer partial sums but too few warps: with blocks
 // that sum 64 columns each the first took 237 us.
 
 constexpr int LONG_JOIN = 8;            // more partial sums than this are shared out among a block's warps
@@ -447,7 +447,8 @@ struct GradOut {
     const int* keys; const int* pos; int n;
     Tokens tokens;
     float* partial; int pitch;                                  // two rows of `pitch` floats a chunk
-    int* joins; int chunks;                                     // numbers of short and long joins, then their chunks from both ends
+    int4* joins; int chunks;                                    // {numbers of short and long joins}, then {chunk, token, chunks after
+                                                                // this one that begin with the token} from both ends
     float fnew, fold;
 };
 
@@ -551,11 +552,19 @@ embedding_sum_kernel(const GradOut<G> o, const T* __restrict__ dout, long long l
     }
     if (ends >> (count - 1) & 1) return;
     store_units<T, float, ALIGNED>(o.partial + (chunk * 2 + (begun_before ? 0 : 1)) * o.pitch, slice, o.units, acc);
-    if (!begun_before && slice == 0 && lane == 31) {            // this chunk's last token is to be joined
-        const long long far = first + (LONG_JOIN + 1) * 32;
-        const bool is_long = far < o.n && o.keys[far] == key;
-        const int place = atomicAdd(&o.joins[is_long], 1);
-        o.joins[2 + (is_long ? o.chunks - 1 - place : place)] = (int)chunk;
+    if (begun_before || slice != 0) return;
+    const int token = __shfl_sync(0xffffffffu, key, 31);        // this chunk's last token is to be joined
+    int more = 0;
+    for (;;) {
+        const long long c = (chunk + 1 + more + lane) * 32;
+        const unsigned same = __ballot_sync(0xffffffffu, c < o.n && o.keys[c] == token);
+        if (same != 0xffffffffu) { more += __ffs(~same) - 1; break; }
+        more += 32;
+    }
+    if (lane == 0) {
+        const bool is_long = more > LONG_JOIN;
+        const int place = atomicAdd(reinterpret_cast<int*>(o.joins) + is_long, 1);
+        o.joins[1 + (is_long ? o.chunks - 1 - place : place)] = make_int4((int)chunk, token, more, 0);
     }
 }
 
@@ -568,16 +577,6 @@ embedding_join_kernel(const GradOut<G> o) {
     __shared__ float4 shares[8][32];
     wait_for_dependencies();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slices = (o.units + 127) / 128;
-    // chunks after this one that begin with the token
-    auto followers = [&](int chunk, int key) {
-        int more = 0;
-        for (;;) {
-            const long long c = ((long long)chunk + 1 + more + lane) * 32;
-            const unsigned same = __ballot_sync(0xffffffffu, c < o.n && o.keys[c] == key);
-            if (same != 0xffffffffu) return more + __ffs(~same) - 1;
-            more += 32;
-        }
-    };
     auto add = [](float4& acc, const float4& x) { acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w; };
     auto finish = [&](int key, int u, const float4& acc) {
         G* to = o.dtable + key * o.ldt;
@@ -586,11 +585,12 @@ embedding_join_kernel(const GradOut<G> o) {
         for (int e = 0; e < 4; e++)
             if (u + e < o.units) to[u + e] = from_f32<G>(o.fold != 0.f ? o.fold * to_f32(to[u + e]) + o.fnew * x[e] : o.fnew * x[e]);
     };
-    const long long n_long = (long long)o.joins[1] * slices, n_short = (long long)o.joins[0] * slices;
+    const int4 numbers = o.joins[0];
+    const long long n_long = (long long)numbers.y * slices, n_short = (long long)numbers.x * slices;
     for (long long item = blockIdx.x; item < n_long; item += gridDim.x) {
-        const int chunk = o.joins[2 + o.chunks - 1 - (int)(item / slices)], u = (int)(item % slices) * 128 + lane * 4;
-        const int key = o.keys[(long long)chunk * 32 + 31], more = followers(chunk, key);
-        const float* row = o.partial + ((long long)chunk * 2 + 2) * o.pitch + u;
+        const int4 join = o.joins[o.chunks - (int)(item / slices)];
+        const int u = (int)(item % slices) * 128 + lane * 4, more = join.z;
+        const float* row = o.partial + ((long long)join.x * 2 + 2) * o.pitch + u;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (u < o.pitch) {
             if (warp == 0) add(acc, *reinterpret_cast<const float4*>(row - o.pitch));
@@ -603,18 +603,18 @@ embedding_join_kernel(const GradOut<G> o) {
         __syncthreads();
         if (warp == 0) {
             for (int w = 1; w < 8; w++) add(acc, shares[w][lane]);
-            finish(key, u, acc);
+            finish(join.y, u, acc);
         }
     }
     for (long long item = (long long)blockIdx.x * 8 + warp; item < n_short; item += (long long)gridDim.x * 8) {
-        const int chunk = o.joins[2 + (int)(item / slices)], u = (int)(item % slices) * 128 + lane * 4;
-        const int key = o.keys[(long long)chunk * 32 + 31], more = followers(chunk, key);
-        const float* row = o.partial + ((long long)chunk * 2 + 2) * o.pitch + u;
+        const int4 join = o.joins[1 + (int)(item / slices)];
+        const int u = (int)(item % slices) * 128 + lane * 4, more = join.z;
+        const float* row = o.partial + ((long long)join.x * 2 + 2) * o.pitch + u;
         if (u >= o.pitch) continue;
         float4 acc = *reinterpret_cast<const float4*>(row - o.pitch);
 #pragma unroll 8
         for (int c = 0; c < more; c++) add(acc, *reinterpret_cast<const float4*>(row + (long long)c * 2 * o.pitch));
-        finish(key, u, acc);
+        finish(join.y, u, acc);
     }
 }
 
@@ -693,7 +693,7 @@ static GradLayout grad_layout(int units, int vocab, int ncols) {
         g.pos[1] = take(4LL * ncols);
         g.counts = take(4LL * SORT_DIGITS * g.tiles);
     }
-    g.joins = take(4LL * (2 + g.chunks));
+    g.joins = take(16LL * (1 + g.chunks));
     g.partial = take(4LL * 2 * g.chunks * g.pitch);
     g.bytes = at;
     return g;
@@ -728,7 +728,7 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     int* keys[2] = {(int*)(ws + g.keys[0]), (int*)(ws + g.keys[1])};
     int* pos[2] = {(int*)(ws + g.pos[0]), (int*)(ws + g.pos[1])};
     int* counts = (int*)(ws + g.counts);
-    int* joins = (int*)(ws + g.joins);
+    int4* joins = (int4*)(ws + g.joins);
     int src = 0, rc = CUVDIA_OK;
     if (g.cluster) {
         int blocks = 1, r = 1;
@@ -779,7 +779,7 @@ int launch_embedding_grad(void* dtable, int ldt, int grad_type, const void* dout
     count_launch();
     rc = check_launch("embedding_sum_kernel");
     if (rc) return rc;
-    const unsigned join_blocks = (unsigned)std::min((g.chunks - 1) * (((long long)units + 127) / 128), 4LL * sm_count());
+    const unsigned join_blocks = (unsigned)std::min((g.chunks - 1) * (((long long)units + 127) / 128), 6LL * sm_count());
     CUVDIA_FLOAT_TYPE(grad_type, {
         const GradOut<T> o = GRAD_OUT(T);
         rc = launch_dependent(embedding_join_kernel<T>, join_blocks, 256, st, o);
