@@ -367,6 +367,30 @@ def test_token_logprob_of_far_logits():
     check_logprob(x, tok, 1.0, 4, r)
 
 
+@pytest.mark.parametrize("vocab, ncols", [(50, 9), (3000, 2000), (40000, 3), (40000, 700)])
+def test_token_logprob_gives_what_is_asked_for(vocab, ncols):
+    """The C entry point with every choice of results; what is not asked for is not written."""
+    from cuv_b200 import _capi
+    x = matrix(gen(3), vocab, ncols, torch.float16, spread=3.0)[0]
+    tok = torch.randint(0, vocab, (ncols,), device="cuda", generator=gen(4), dtype=torch.int32)
+    all_of_them = cb.token_logprob(x, tok, scale=0.5, entropy=True, top=7)
+    for choice in range(1, 16):
+        logp, lse, ent = (torch.full((ncols,), 9.0, device="cuda") for _ in range(3))
+        top_logp, top_index = torch.full((ncols, 7), 9.0, device="cuda"), torch.full((ncols, 7), 9, dtype=torch.int32, device="cuda")
+        want = [choice >> k & 1 for k in range(4)]
+        rc = _capi.lib().cuvdia_token_logprob(
+            x.data_ptr(), vocab, _capi.T_F16, vocab, ncols, tok.data_ptr() if want[0] else None, _capi.T_I32, 0.5,
+            logp.data_ptr() if want[0] else None, lse.data_ptr() if want[1] else None, ent.data_ptr() if want[2] else None,
+            7 if want[3] else 0, top_logp.data_ptr() if want[3] else None, top_index.data_ptr() if want[3] else None,
+            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        check_logprob(x, tok, 0.5, 7 if want[3] else 0, cb.TokenLogprob(
+            logp if want[0] else all_of_them.logp, lse if want[1] else all_of_them.lse, ent if want[2] else None,
+            top_logp.t(), top_index.t()))
+        for t, w in ((logp, want[0]), (lse, want[1]), (ent, want[2]), (top_logp, want[3]), (top_index, want[3])):
+            assert w or (t == 9).all()
+
+
 # ---- gradient of the log probabilities ------------------------------------------------------------------------------
 
 def check_grad(dlogits, logits, lse, tok, dlogp, entropy, dentropy, scale):
