@@ -368,12 +368,12 @@ struct LogprobArgs {
     float* top_logp; int* top_index;
 };
 
-// The results of a column from its statistics and its descending list: one warp.  given: the column's token is one of the
-// vocabulary; given_logit is its logit then.
-template <class T, bool ENT, bool TOP>
+// The results of a column from its statistics and its descending list: LANES neighbouring lanes.  given: the column's token is
+// one of the vocabulary; given_logit is its logit then.
+template <class T, bool ENT, bool TOP, int LANES>
 __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col, bool given, float given_logit, const Stat& a,
                                              Key list) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x % LANES;
     const bool none = a.m == -INFINITY && a.s == 0.f;
     const float m0 = shift(a.m), l2s = log2f(a.s);
     if (lane == 0) {
@@ -387,8 +387,8 @@ __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col
     }
 }
 
-// TEAM threads share a column's part: a whole block, or a warp (eight columns a block of 256) where a column is so short
-// that a block's joins would cost more than its elements.  A cluster of `parts` blocks shares a column where the columns
+// TEAM threads share a column's part: a whole block, or a warp or eight lanes (8 or 32 columns a block of 256) where a column
+// is so short that a block's joins, or a warp's, would cost more than its elements.  A cluster of `parts` blocks shares a column where the columns
 // alone are too few to fill the GPU: its blocks leave their sums and lists in the first block's shared memory, which joins
 // them, so that there is one launch and no scratch memory.
 //
@@ -396,11 +396,12 @@ __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col
 // 50021 x 1000 f32 39 us (5.1 TB/s: 7 blocks on most SMs, 6 on the others, and their common start and end), with 20 alternatives
 // and a third of the tokens forbidden 45 us.  A few columns are bound by latency: 131072 x 4 bf16 6 us, 8.5 us with alternatives.
 template <class T, bool ENT, bool TOP, int TEAM>
-__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM, TEAM == 128 ? 8 : 4)
+__global__ void __launch_bounds__(TEAM < 128 ? 256 : TEAM, TEAM == 128 ? 8 : 4)
 token_logprob_kernel(const LogprobArgs q, int parts) {
-    constexpr int V = Vec16<T>::N, THREADS = TEAM == 32 ? 256 : TEAM, WARPS = TEAM == 32 ? 8 : TEAM / 32, STEP = TEAM;
+    constexpr int V = Vec16<T>::N, THREADS = TEAM < 128 ? 256 : TEAM, WARPS = THREADS / 32, LANES = TEAM < 32 ? TEAM : 32, STEP = TEAM;
     constexpr int STAGES = TEAM == 128 && !TOP ? 3 : 2;          // three would not leave room for a list's arrays in as many blocks
-    constexpr bool BLOCK = TEAM != 32;
+    constexpr bool BLOCK = TEAM >= 128;
+    static_assert(TEAM >= 32 || (TEAM >= V - 1 && !TOP), "lists and ends");
     __shared__ uint4 ring[STAGES * U * THREADS];
     __shared__ Stat stats[WARPS], part_stats[8];
     __shared__ Key lists[TOP ? WARPS : 1][32], part_lists[TOP ? 8 : 1][32], buffers[TOP ? WARPS : 1][64];
@@ -408,12 +409,14 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     __shared__ int found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = BLOCK ? blockIdx.x % (unsigned)parts : 0;
-    const long long col = BLOCK ? blockIdx.x / (unsigned)parts : (long long)blockIdx.x * WARPS + warp;
+    long long col = BLOCK ? blockIdx.x / (unsigned)parts : (long long)blockIdx.x * (THREADS / TEAM) + threadIdx.x / TEAM;
     if (BLOCK && parts > 1) cluster_arrive();             // waited for before the first remote store: all blocks run then
-    if (col >= q.ncols) return;
+    const bool beyond = col >= q.ncols;
+    if (beyond && TEAM >= 32) return;
+    if (beyond) col = q.ncols - 1;                              // for the other lanes' shuffles; nothing is written
     const T* x0 = (const T*)q.logits + col * q.ld;
     const float c = q.scale * LOG2E;
-    const int tid = BLOCK ? threadIdx.x : lane;
+    const int tid = threadIdx.x % TEAM;
     // whole 16-byte vectors of the column, behind `head` elements and before the rest
     const int head = min(q.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)));
     const int nvec = (q.vocab - head) / V, rest = q.vocab - head - nvec * V;
@@ -425,7 +428,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     // the given token's logit, fetched here so that it need not be waited for at the end
     bool given = false;
     float given_logit = 0.f;
-    if (q.logp && lane == 0 && part == 0 && (!BLOCK || warp == 0)) {
+    if (q.logp && tid == 0 && part == 0) {
         const long long t = q.tokens[col];
         given = t >= 0 && t < q.vocab;
         if (given) given_logit = to_f32(x0[t]);
@@ -461,15 +464,23 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
     const float largest = a.m;
     float edge = -INFINITY;                                     // of the ends: one element a lane at most
     int edge_at = -1;
-    if (part == 0 && (!BLOCK || warp == 0) && head + rest > 0) {       // the ends, element by element
-        edge_at = lane < head ? lane : lane >= 16 && lane - 16 < rest ? head + nvec * V + lane - 16 : -1;
-        edge = edge_at >= 0 ? to_f32(x0[edge_at]) : -INFINITY;
+    auto add_edge = [&](int at) {
+        edge_at = at;
+        edge = at >= 0 ? to_f32(x0[at]) : -INFINITY;
         Stat b = {fmaxf(edge, -INFINITY), 0.f, 0.f};            // NaN: leaves the maximum to the others
         const float d = (edge - shift(b.m)) * c;
         b.s = exp2_approx(d);
         b.t = b.s * fmaxf(d, LEAST);
         const Stat joined = merge({a.m, a.s.x + a.s.y, a.t.x + a.t.y}, b, c);
         a = {joined.m, {joined.s, 0.f}, {joined.t, 0.f}};
+    };
+    if (part == 0 && (!BLOCK || warp == 0) && head + rest > 0) {       // the ends, element by element
+        if (TEAM >= 32) {
+            add_edge(lane < head ? lane : lane >= 16 && lane - 16 < rest ? head + nvec * V + lane - 16 : -1);
+        } else {
+            add_edge(tid < head ? tid : -1);
+            add_edge(tid < rest ? head + nvec * V + tid : -1);
+        }
     }
     Key list = 0;
     if (TOP) {
@@ -521,8 +532,11 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
             }
         }
     }
-    Stat st = join_lanes<ENT, 32>({a.m, a.s.x + a.s.y, ENT ? a.t.x + a.t.y : 0.f}, c);
-    if (!BLOCK) { write_column<T, ENT, TOP>(q, col, given, given_logit, st, list); return; }
+    Stat st = join_lanes<ENT, LANES>({a.m, a.s.x + a.s.y, ENT ? a.t.x + a.t.y : 0.f}, c);
+    if (!BLOCK) {
+        if (!beyond) write_column<T, ENT, TOP, LANES>(q, col, given, given_logit, st, list);
+        return;
+    }
 
     if (lane == 0) stats[warp] = st;
     __syncthreads();
@@ -546,7 +560,7 @@ token_logprob_kernel(const LogprobArgs q, int parts) {
             list = merge_warps(list, lists, parts);
         }
     }
-    if (warp == 0) write_column<T, ENT, TOP>(q, col, given, given_logit, st, list);
+    if (warp == 0) write_column<T, ENT, TOP, LANES>(q, col, given, given_logit, st, list);
 }
 
 template <class T, bool ENT, bool TOP>
@@ -555,6 +569,13 @@ static int logprob_go(const LogprobArgs& q, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(256);
     cfg.stream = st;
+    // eight lanes a column where it is short (304 x 20000 bf16: 10.3 us, by warps 20 us; 1024 x 20000: 14.5 and 19 us, but
+    // 2048 x 4000: 10.2 and 8.2 us), if there are enough of them (304 x 1000: 5.6 us, by blocks 7.4 us)
+    if (!TOP && nvec <= 128 && q.ncols >= 4 * sm_count()) {
+        cfg.gridDim = dim3((unsigned)(((long long)q.ncols + 31) / 32));
+        CUVDIA_CUDA(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T, ENT, false, 8>, q, 1));
+        return CUVDIA_OK;
+    }
     // a warp a column (8000 x 8000 bf16: 29 us, by blocks 35 us), if there are enough of them (8000 x 700: 8.2 us, by blocks 7.1 us)
     if (nvec <= 1024 && q.ncols >= 8 * sm_count()) {
         cfg.gridDim = dim3(((unsigned)q.ncols + 7) / 8);

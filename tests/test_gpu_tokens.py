@@ -247,8 +247,9 @@ def plain_logprob(logits, tokens, scale):
     """In 64 bits: lse, logp, entropy, log probabilities, and the mean of |log2 p / pmax| that bounds count with."""
     z = logits.double() * float(np.float32(scale))
     m = z.amax(0).nan_to_num(neginf=0.0)
-    lse = m + torch.log(torch.exp(z - m).sum(0))
-    logq = torch.where(lse == -math.inf, -math.inf, z - lse)
+    logs = torch.log(torch.exp(z - m).sum(0))
+    lse = m + logs
+    logq = torch.where(lse == -math.inf, -math.inf, (z - m) - logs)     # z - lse loses logs where m is f32's lowest value
     q = torch.exp(logq)
     ent = -(q * torch.where(q == 0, 0.0, logq)).sum(0)
     vocab = logits.shape[0]
@@ -356,6 +357,38 @@ def test_token_logprob_masks_ties_and_specials(kind, vocab, ncols):
     left = z[:, 0].float().clone()
     left[vocab // 3] = -math.inf
     assert r.top_index[0, 0] == left.argmax()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab, ld, offset", [(1, None, 0), (3, 5, 1), (50, 50, 3), (256, None, 0), (509, 509, 5), (512, 1000, 0),
+                                               (515, 515, 1), (1023, 1023, 7), (1031, 1031, 2)])
+@pytest.mark.parametrize("ncols", [591, 593, 2111])
+def test_token_logprob_of_many_short_columns(kind, vocab, ld, offset, ncols):
+    g, dtype = gen(vocab + ncols), TYPES[kind]
+    x, buf = matrix(g, vocab, ncols, dtype, ld, offset, spread=4.0)
+    tok = torch.randint(-1, vocab + 1, (ncols,), device="cuda", generator=g)
+    keep = buf.clone()
+    check_logprob(x, tok, 1.0, 0, cb.token_logprob(x, tok, entropy=True))
+    check_logprob(x, tok, 0.3, 0, cb.token_logprob(x, tok.int(), scale=0.3))
+    assert torch.equal(buf.nan_to_num(7.0), keep.nan_to_num(7.0))
+    # forbidden tokens, the type's lowest value, columns without a token left, NaN and +inf in single columns
+    x[torch.rand(vocab, ncols, device="cuda", generator=g) < 0.4] = -math.inf
+    x[torch.rand(vocab, ncols, device="cuda", generator=g) < 0.05] = torch.finfo(dtype).min
+    x[:, 7] = -math.inf
+    x[:, -1] = -math.inf
+    want = cb.token_logprob(x, tok, entropy=True)
+    check_logprob(x, tok, 1.0, 0, want)
+    assert want.lse[-1] == -math.inf and want.entropy[7] == 0
+    x[vocab // 2, 3] = math.nan
+    x[vocab - 1, 12] = math.inf
+    r = cb.token_logprob(x, tok, entropy=True)
+    there = (tok >= 0) & (tok < vocab)
+    for name in ("lse", "logp", "entropy"):
+        a, b = getattr(r, name).clone(), getattr(want, name)
+        for col in (3, 12):
+            assert torch.isnan(a[col]) or name == "logp" and not there[col]
+            a[col] = b[col]
+        assert torch.equal(a, b)
 
 
 def test_token_logprob_of_far_logits():
