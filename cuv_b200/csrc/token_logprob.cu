@@ -631,8 +631,9 @@ int launch_token_logprob(const void* logits, int ld, int type, int vocab, int nc
 //   dlogits_v = scale * (dlogp * ([v = token] - p_v) - dentropy * p_v * (log p_v + entropy)),   p_v = exp(scale * logit_v - lse)
 // Element-wise once lse and entropy are known: with d = scale * logit - lse,
 //   dlogits_v = 2^(d log2 e) * (A d + B) (+ scale * dlogp at the token),   A = -scale dentropy,  B = -scale (dlogp + dentropy entropy)
-// two elements an instruction.  A block owns up to 1024 vectors of one column, those of the logits' memory; the stores are vectors
-// too where dlogits lies alike, else element by element.  In place is fine: a thread reads its elements before it writes them.
+// two elements an instruction.  A block owns up to 1024 vectors of one column, those of the logits' memory; 16 lanes own all of
+// a column of up to 64.  The stores are vectors too where dlogits lies alike, else element by element.  In place is fine: a
+// thread reads its elements before it writes them.
 // Bound by memory: 32768 x 8192 bf16 with or without entropies 158 us (6.8 TB/s), 32768 x 4096 f32 160 us.  The straight-line path
 // for blocks that lie inside a column is what that took (one path with tests per vector: 176 us).
 struct GradFactors { float scale, minus_lse, a, b; };
@@ -655,14 +656,17 @@ __device__ __forceinline__ void grad_vector(float (&x)[Vec16<T>::N], const GradF
     for (int e = 0; e < Vec16<T>::N; e += 2) grad_pair<ENT, CUT>(x[e], x[e + 1], f);
 }
 
-template <class T, bool ENT, int THREADS>
-__global__ void __launch_bounds__(THREADS)
-token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long ld, int vocab, const Tokens tokens, float scale,
+template <class T, bool ENT, int TEAM>
+__global__ void __launch_bounds__(TEAM < 64 ? 256 : TEAM)
+token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long ld, int vocab, int ncols, const Tokens tokens, float scale,
                           const float* __restrict__ lse, const float* __restrict__ dlogp, const float* __restrict__ entropy,
                           const float* __restrict__ dentropy, int chunks) {
     constexpr int V = Vec16<T>::N;
-    const long long col = blockIdx.x / (unsigned)chunks;
-    const int chunk = blockIdx.x - (unsigned)col * (unsigned)chunks;
+    constexpr bool SHORT = TEAM < 64;                           // several columns a block
+    const int tid = threadIdx.x % TEAM;
+    const long long col = SHORT ? (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM : blockIdx.x / (unsigned)chunks;
+    const int chunk = SHORT ? 0 : blockIdx.x - (unsigned)col * (unsigned)chunks;
+    if (SHORT && col >= ncols) return;
     const T* x0 = logits + col * ld;
     T* y0 = dlogits + col * ldd;
     // whole vectors of the column, behind `head` elements and before the rest
@@ -677,12 +681,12 @@ token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long 
     const bool zero = (t < 0 && !ENT) || l == -INFINITY;
     const uint4* from = reinterpret_cast<const uint4*>(x0 + head);
     T* to = y0 + head;
-    const int v0 = chunk * (THREADS * U) + (int)threadIdx.x;
-    const bool plain = alike && !zero && (chunk + 1) * (THREADS * U) <= nvec;           // as most blocks are
+    const int v0 = chunk * (TEAM * U) + tid;
+    const bool plain = !SHORT && alike && !zero && (chunk + 1) * (TEAM * U) <= nvec;    // as most blocks are
     uint4 raw[U];
     if (plain) {
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = from[v0 + u * THREADS];
+        for (int u = 0; u < U; u++) raw[u] = from[v0 + u * TEAM];
     }
     const float g = t >= 0 ? dlogp[col] : 0.f, h = ENT ? dentropy[col] : 0.f, hot = scale * g;
     const GradFactors f = {scale, -l, -scale * h, -scale * (ENT ? fmaf(h, entropy[col], g) : g)};
@@ -702,10 +706,16 @@ token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long 
     };
     if (plain) {
 #pragma unroll
-        for (int u = 0; u < U; u++) reinterpret_cast<uint4*>(to)[v0 + u * THREADS] = whole_vector(raw[u], v0 + u * THREADS);
+        for (int u = 0; u < U; u++) reinterpret_cast<uint4*>(to)[v0 + u * TEAM] = whole_vector(raw[u], v0 + u * TEAM);
+    } else if (SHORT && alike && !zero) {
+#pragma unroll
+        for (int u = 0; u < U; u++) if (v0 + u * TEAM < nvec) raw[u] = from[v0 + u * TEAM];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (v0 + u * TEAM < nvec) reinterpret_cast<uint4*>(to)[v0 + u * TEAM] = whole_vector(raw[u], v0 + u * TEAM);
     } else {
 #pragma unroll 1
-        for (int v = v0; v < min(nvec, (chunk + 1) * (THREADS * U)); v += THREADS) {
+        for (int v = v0; v < min(nvec, (chunk + 1) * (TEAM * U)); v += TEAM) {
             const uint4 r = zero ? make_uint4(0, 0, 0, 0) : whole_vector(from[v], v);
             if (alike) { reinterpret_cast<uint4*>(to)[v] = r; continue; }
             float x[V];
@@ -714,8 +724,9 @@ token_logprob_grad_kernel(T* dlogits, long long ldd, const T* logits, long long 
             for (int e = 0; e < V; e++) to[v * V + e] = from_f32<T>(x[e]);
         }
     }
-    if (chunk == 0 && (int)threadIdx.x < head + rest) {         // the ends, one element a thread
-        const int i = (int)threadIdx.x < head ? (int)threadIdx.x : nvec * V + (int)threadIdx.x;
+    static_assert(TEAM >= 2 * (V - 1), "ends");
+    if (chunk == 0 && tid < head + rest) {                      // the ends, one element a thread
+        const int i = tid < head ? tid : nvec * V + tid;
         float x[2] = {zero ? 0.f : to_f32(x0[i]), 0.f};
         if (!zero) grad_pair<ENT, true>(x[0], x[1], f);
         y0[i] = from_f32<T>(zero ? 0.f : t == i ? x[0] + hot : x[0]);
@@ -726,16 +737,19 @@ int launch_token_logprob_grad(void* dlogits, int ldd, const void* logits, int ld
                               const void* tokens, int token_type, float scale, const float* lse, const float* dlogp,
                               const float* entropy, const float* dentropy, cudaStream_t st) {
     const int v = 16 / type_size(type);
-    // blocks of 1024 vectors, of 256 where a column has no more (1000 x 4000 bf16: 8.2 us, with large blocks 12.3 us)
-    const int threads = vocab > 256 * v ? 256 : 64;
-    const long long chunks = std::max(1LL, ((long long)vocab / v + threads * U - 1) / (threads * U));
-    const long long blocks = chunks * ncols;
+    // blocks of 1024 vectors, of 256 where a column has no more (1000 x 4000 bf16: 8.2 us, with large blocks 12.3 us); 16 lanes a
+    // column where columns are short (305 x 100000 bf16: 31 us, by blocks 59 us; 512 x 20000: 12.3 and 16.4 us, but 1024 x 1000:
+    // 5.3 and 4.4 us) and more than the SMs hold at a time (below that the two take the same)
+    const int team = vocab > 256 * v ? 256 : vocab > 64 * v || ncols < 4 * sm_count() ? 64 : 16;
+    const long long chunks = std::max(1LL, ((long long)vocab / v + team * U - 1) / (team * U));
+    const long long blocks = team == 16 ? ((long long)ncols + 15) / 16 : chunks * ncols;
     if (blocks > 2147483647LL) { set_last_error("token_logprob_grad: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
-#define LG_GO(E, N) token_logprob_grad_kernel<T, E, N><<<(unsigned)blocks, N, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld, \
-    vocab, make_tokens(tokens, token_type), scale, lse, dlogp, entropy, dentropy, (int)chunks)
+#define LG_GO(E, N) token_logprob_grad_kernel<T, E, N><<<(unsigned)blocks, N < 64 ? 256 : N, 0, st>>>((T*)dlogits, ldd, (const T*)logits, ld, \
+    vocab, ncols, make_tokens(tokens, token_type), scale, lse, dlogp, entropy, dentropy, (int)chunks)
     CUVDIA_FLOAT_TYPE(type, {
-        if (threads == 256) { if (dentropy) LG_GO(true, 256); else LG_GO(false, 256); }
-        else                { if (dentropy) LG_GO(true, 64); else LG_GO(false, 64); }
+        if (team == 256)     { if (dentropy) LG_GO(true, 256); else LG_GO(false, 256); }
+        else if (team == 64) { if (dentropy) LG_GO(true, 64); else LG_GO(false, 64); }
+        else                 { if (dentropy) LG_GO(true, 16); else LG_GO(false, 16); }
     });
 #undef LG_GO
     count_launch();

@@ -486,6 +486,37 @@ def test_token_logprob_grad(kind, vocab, ld, offset, ncols):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab, ld, offset", [(1, None, 0), (3, 5, 1), (50, 50, 3), (256, None, 0), (257, 257, 5), (512, 1000, 0),
+                                               (509, 509, 7), (515, 515, 1)])
+@pytest.mark.parametrize("ncols", [591, 593, 2111])
+def test_token_logprob_grad_of_many_short_columns(kind, vocab, ld, offset, ncols):
+    g, dtype = gen(vocab + ncols), TYPES[kind]
+    x = matrix(g, vocab, ncols, dtype, ld, offset, spread=3.0)[0]
+    tok = torch.randint(-1, vocab + 1, (ncols,), device="cuda", generator=g)
+    dlogp, dent = torch.randn(ncols, device="cuda", generator=g), torch.randn(ncols, device="cuda", generator=g)
+    dlogp[tok < 0] = math.nan                                   # not used
+    for masked in (False, True):
+        if masked:
+            x[torch.rand(vocab, ncols, device="cuda", generator=g) < 0.4] = -math.inf
+            x[:, 7] = -math.inf
+            x[:, -1] = -math.inf
+        r = cb.token_logprob(x, tok, scale=0.7, entropy=True)
+        for a, e, b in ((dlogp, None, None), (None, r.entropy, dent), (dlogp, r.entropy, dent)):
+            d, buf = matrix(g, vocab, ncols, dtype, ld, offset, fill=5.0)
+            cb.token_logprob_grad(d, x, r.lse, tok if a is not None else None, a, e, b, 0.7)
+            check_grad(d, x, r.lse, tok, a, e, b, 0.7)
+            outside_untouched(buf, d)
+        other, buf = matrix(g, vocab, ncols, dtype, vocab + 3, 2, fill=5.0)         # another alignment, and in place
+        cb.token_logprob_grad(other, x, r.lse, tok, dlogp, r.entropy, dent, 0.7)
+        outside_untouched(buf, other)
+        y, buf = matrix(g, vocab, ncols, dtype, ld, offset, fill=0.0)
+        y.copy_(x)
+        cb.token_logprob_grad(y, y, r.lse, tok, dlogp, r.entropy, dent, 0.7)
+        assert torch.equal(y, d) and torch.equal(other, d)
+        outside_untouched(buf, y)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_token_logprob_grad_masks(kind):
     g, dtype, vocab = gen(5), TYPES[kind], 3003
     x = matrix(g, vocab, 4, dtype, spread=2.0)[0]
