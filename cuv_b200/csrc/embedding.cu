@@ -14,7 +14,7 @@ namespace cuvdia {
 // and shifted into place, so that only the ends of a column are moved element by element.  Bound by memory: 4096 x 32768 bf16 from
 // a table of 65536 tokens, text-like frequencies, 61 us (5.8 TB/s of columns read once and written); 4095 x 32768 84 us (element
 // by element 145 us).  Four vectors a thread (two: 64 us), two where they are shifted (four: 90 us).
-template <class T, bool ALIGNED, bool WIDE>
+template <class T, bool ALIGNED, bool WIDE, bool SPREAD>
 __global__ void __launch_bounds__(256)
 embedding_kernel(T* __restrict__ dst, long long ldd, const T* __restrict__ table, long long ldt, int units, int vocab,
                  const Tokens tokens, int ncols, float scale, int log_lanes, int parts) {
@@ -37,6 +37,17 @@ embedding_kernel(T* __restrict__ dst, long long ldd, const T* __restrict__ table
     T* to = dst + col * ldd;
     const int i0 = (part * lanes * U + l) * E - (ALIGNED ? 0 : behind16(to));
     const int r = ALIGNED ? 0 : behind16(from + i0);            // the same for all of a column's vectors
+    // SPREAD: the elements below `front` and from `back` on, which no vector moves, fewer than 4 E, are moved by the last part's
+    // threads, one each where there are 32.
+    int front = 0, back = 0, ends = 0;
+    T end;
+    if (SPREAD) {
+        const int low = there ? r : 0, high = units - E - (there && r ? E - r : 0), behind = behind16(to);  // first vectors' places
+        front = min(units, (low + behind + E - 1) / E * E - behind);
+        back = high >= front ? front + ((high - front) / E + 1) * E : front;
+        if (part == parts - 1) ends = front + units - back;
+        if (l < ends && there) end = from[l < front ? l : back + l - front];
+    }
     uint4 raw[U], more[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -64,10 +75,17 @@ embedding_kernel(T* __restrict__ dst, long long ldd, const T* __restrict__ table
                 raw[u] = pack16<T>(x);
             }
             *reinterpret_cast<uint4*>(to + i) = raw[u];
-        } else {
+        } else if (!SPREAD) {
 #pragma unroll
             for (int e = 0; e < E; e++)
                 if (i + e >= 0 && i + e < units) to[i + e] = from_f32<T>(there ? to_f32(from[i + e]) * scale : 0.f);
+        }
+    }
+    if (SPREAD) {
+        if (l < ends) to[l < front ? l : back + l - front] = from_f32<T>(there ? to_f32(end) * scale : 0.f);
+        for (int k = l + lanes; k < ends; k += lanes) {
+            const int i = k < front ? k : back + k - front;
+            to[i] = from_f32<T>(there ? to_f32(from[i]) * scale : 0.f);
         }
     }
 }
@@ -89,8 +107,16 @@ static int embedding_go(T* dst, int ldd, const T* table, int ldt, int units, int
     const long long blocks = log_lanes == 8 ? parts : (teams + (256 >> log_lanes) - 1) >> (8 - log_lanes);
     if (teams > 4294967295LL || blocks > 2147483647LL) { set_last_error("embedding: %lld blocks", blocks); return CUVDIA_ERR_UNSUPPORTED; }
     const dim3 grid((unsigned)blocks, log_lanes == 8 ? (unsigned)y : 1, log_lanes == 8 ? (unsigned)((ncols + y - 1) / y) : 1);
-    if (log_lanes == 8) embedding_kernel<T, ALIGNED, true><<<grid, 256, 0, st>>>(dst, ldd, table, ldt, units, vocab, tokens, ncols, scale, log_lanes, (int)parts);
-    else embedding_kernel<T, ALIGNED, false><<<grid, 256, 0, st>>>(dst, ldd, table, ldt, units, vocab, tokens, ncols, scale, log_lanes, (int)parts);
+#define LOOKUP_GO(W, S) \
+    embedding_kernel<T, ALIGNED, W, S><<<grid, 256, 0, st>>>(dst, ldd, table, ldt, units, vocab, tokens, ncols, scale, log_lanes, (int)parts)
+    // Shorter 16-bit columns have their ends spread over the threads (333 x 32000 bf16: 14 us, each vector by its own thread
+    // 22 us; 1023: 31 and 35 us), which the others do better without (5001 x 32000 bf16: 92 us, spread 100 us; 1023 x 32000 f32:
+    // 41 and 45 us).
+    constexpr bool ENDS = !ALIGNED && sizeof(T) == 2;
+    if (log_lanes == 8) LOOKUP_GO(true, false);
+    else if (ENDS && units < 2048) LOOKUP_GO(false, ENDS);
+    else LOOKUP_GO(false, false);
+#undef LOOKUP_GO
     count_launch();
     return check_launch("embedding_kernel");
 }

@@ -83,6 +83,21 @@ def test_embedding(kind, units, ld, offset, ncols):
         outside_untouched(buf, dst)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("units", [*range(1, 42), 63, 64, 65, 127, 255, 257, 333, 511, 767, 1023, 1025, 1534, 2047, 2049])
+def test_embedding_of_short_columns_that_lie_differently(kind, units):
+    """Whole columns come out bit for bit, whatever the alignment of either side."""
+    g, dtype, vocab, ncols = gen(units), TYPES[kind], 19, 41
+    tok = torch.randint(-1, vocab + 1, (ncols,), device="cuda", generator=g)
+    there = (tok >= 0) & (tok < vocab)
+    for shift, ld_from, ld_to in ((0, units, units), (3, units + 1, units + 2), (5, units + 3, units), (7, units, units + 5)):
+        table, _ = matrix(g, units, vocab, dtype, ld_from, shift)
+        dst, buf = matrix(g, units, ncols, dtype, ld_to, 7 - shift, fill=5.0)
+        cb.embedding(dst, table, tok)
+        assert torch.equal(dst, torch.where(there, table[:, tok.clamp(0, vocab - 1)], 0.0))
+        outside_untouched(buf, dst)
+
+
 def test_embedding_copies_bits_and_reads_no_other_column():
     table = torch.full((5, 64), math.nan, device="cuda").t()
     table[:, 3] = torch.tensor([0.0, -0.0, math.inf, -math.inf] * 16, device="cuda")
