@@ -1,13 +1,14 @@
 // Thread-block clusters: the hardware's barrier over a cluster's blocks (which are scheduled together, so it always ends), and
 // addresses in another block's shared memory.
+//
+// An arrival releases: what the thread did before it, reads of other blocks' shared memory included, is done for the threads that
+// leave the wait.  (A relaxed arrival would order nothing: a block whose shared memory is still being read could end.)
 #pragma once
 #include "cuvdia_internal.cuh"
 
 namespace cuvdia {
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-// for blocks that only tell each other how far they are, with nothing written to be seen
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // the address, in block `rank` of the cluster, of the variable that this block sees at p

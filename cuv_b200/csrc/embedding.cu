@@ -223,7 +223,7 @@ sort_cluster_kernel(const Tokens tokens, int n, int vocab, int passes, int digit
             for (unsigned c = 0; c < 8; c++) { all += v[c]; if (c < rank_in) below += v[c]; }
         }
         const bool last = pass + 1 == passes;
-        if (last) cluster_arrive_relaxed();                     // this block has read the others' counts: they may leave
+        if (last) cluster_arrive();                             // this block's reads of the others' counts are done: they may leave
         if (warp < 16) {                                        // exclusive scan over the digits
             int run = all;
 #pragma unroll

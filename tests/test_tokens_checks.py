@@ -1,6 +1,7 @@
 """Refusals of the token-model operators (column lookup by token, dropout, token log probabilities, their gradients): what the
 C entry points and the Python layer turn away before anything touches a device."""
 import ctypes
+import os
 
 import pytest
 import torch
@@ -165,3 +166,15 @@ def test_calls_run_on_their_tensors_device(monkeypatch):
     cb._call(0, "entry", 7)
     cb._call(2, "entry", 8)
     assert seen == [(7, 1000), ("enter", 2), (8, 1002), ("leave", 2)]
+
+
+def test_cluster_barriers_order_what_came_before_them():
+    """A block that has arrived may be read from no longer once the others leave the wait: every arrival releases, every wait
+    acquires (a relaxed arrival orders no earlier read of another block's shared memory)."""
+    import re
+    from cuv_b200 import build
+    found = []
+    for name in sorted(os.listdir(build.CSRC)):
+        with open(os.path.join(build.CSRC, name)) as f:
+            found += re.findall(r"barrier\.cluster\.[a-z.]+", f.read())
+    assert set(found) == {"barrier.cluster.arrive.release.aligned", "barrier.cluster.wait.acquire.aligned"}
