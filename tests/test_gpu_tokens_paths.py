@@ -2,12 +2,17 @@
 gradients in recorded graphs, on side streams and in tables beyond 2^31 elements, log probabilities by warps, blocks and
 clusters over masks, ties and specials."""
 import math
+import os
+import subprocess
+import sys
 
+import numpy as np
 import pytest
 import torch
 
 import cuv_b200 as cb
-from test_gpu_tokens import gen
+from oracle import host_oracle as ho
+from test_gpu_tokens import E32, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +52,133 @@ def test_every_cluster_of_the_sort_beside_other_work(ncols, vocab):
     torch.cuda.synchronize()
     for dtable in got:
         assert torch.equal(dtable.double(), want)
+
+
+@pytest.mark.parametrize("ncols", [700, 5000, 40000, 140000])
+@pytest.mark.parametrize("fold", [0.0, 1.0])
+def test_sorted_gradients_recorded_on_side_streams(ncols, fold):
+    """Two graphs recorded on a side stream, replayed at the same time on streams of their own, on contents that are not those
+    of the recording: the sort, its dependent sums and joins, a workspace each.  Whole numbers: equality."""
+    units, vocab = 40, 5003
+
+    def operands(seed):
+        g = gen(seed)
+        return text_tokens(g, vocab, ncols), torch.randint(-30, 31, (ncols, units), device="cuda", generator=g).float().t()
+
+    side, made = torch.cuda.Stream(), []
+    for seed in (1, 2):
+        (tok, dout), dtable = operands(seed), torch.ones((vocab, units), device="cuda").t()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            cb.embedding_grad(dtable, tok, dout, 1.0, fold)
+        made.append((graph, tok, dout, dtable))
+    torch.cuda.synchronize()
+    for k, (graph, tok, dout, dtable) in enumerate(made):
+        t, d = operands(11 + k)
+        tok.copy_(t)
+        dout.copy_(d)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(3):
+        for s, m in zip(streams, made):
+            with torch.cuda.stream(s):
+                m[0].replay()
+    torch.cuda.synchronize()
+    for graph, tok, dout, dtable in made:
+        once = whole_sums(tok, dout, vocab)
+        assert torch.equal(dtable.double(), 3 * once + 1.0 if fold else once)
+    # and without a graph, on a side stream of which the current one knows nothing
+    tok, dout = operands(21)
+    dtable = torch.ones((vocab, units), device="cuda").t()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cb.embedding_grad(dtable, tok, dout, 1.0, fold)
+    side.synchronize()
+    assert torch.equal(dtable.double(), whole_sums(tok, dout, vocab) + (1.0 if fold else 0.0))
+
+
+@pytest.mark.parametrize("ncols", [2000, 30000, 135000])
+def test_a_sorted_gradient_recorded_on_its_very_first_call(ncols):
+    """A process whose first call is the recorded one: what the sort needs set for its shared memory is set there."""
+    code = """
+import torch, cuv_b200 as cb
+ncols = %d
+dout = (torch.arange(ncols * 24, device="cuda") %% 17 - 8).float().view(ncols, 24).t()
+tok = torch.arange(ncols, device="cuda") * 7919 %% 1009
+dtable = cb.colmajor_empty(24, 1500)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    cb.embedding_grad(dtable, tok, dout)
+graph.replay()
+torch.cuda.synchronize()
+want = torch.zeros((1500, 24), dtype=torch.float64, device="cuda")
+want.index_add_(0, tok, dout.t().double())
+assert torch.equal(dtable.double(), want.t())
+print("same")
+""" % ncols
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "same", run.stderr[-2000:]
+
+
+def test_sorted_gradients_beyond_32_bits():
+    """A table, and then a batch, of more than 2^31 elements: the far end of either, absent columns there included."""
+    units, vocab, ncols = 65536, 33000, 400
+    g = gen(8)
+    dout = torch.randint(-9, 10, (ncols, units), device="cuda", generator=g, dtype=torch.int8).to(torch.bfloat16).t()
+    tok = torch.full((ncols,), -1, device="cuda")
+    tok[:300] = vocab - 1 - torch.randint(0, 6, (300,), device="cuda", generator=g) * 2
+    tok[300:350] = vocab - 40                                   # whose sums reach over chunks
+    dtable = torch.full((vocab, units), 7.0, dtype=torch.bfloat16, device="cuda").t()
+    cb.embedding_grad(dtable, tok, dout)
+    rows = torch.where(tok < 0, 0, tok - (vocab - 40))
+    want = torch.zeros((40, units), dtype=torch.float64, device="cuda")
+    want.index_add_(0, rows[tok >= 0], dout.t().double()[tok >= 0])
+    assert torch.equal(dtable[:, -40:], want.t().to(torch.bfloat16))                             # below 2^24: one rounding
+    assert (dtable[:, :-40] == 0).all()
+    del dtable
+    ncols, vocab = 33000, 50
+    big = torch.zeros((ncols, units), dtype=torch.bfloat16, device="cuda").t()
+    big[:, -400:] = dout
+    tok = torch.arange(ncols, device="cuda") % vocab
+    dtable = cb.embedding_grad(cb.colmajor_empty(units, vocab), tok, big)
+    want = torch.zeros((vocab, units), dtype=torch.float64, device="cuda")
+    want.index_add_(0, tok[-400:], dout.t().double())
+    assert torch.equal(dtable.double(), want.t())
+
+
+def test_a_token_model_of_many_positions():
+    """Embedding, dropout, a DIA layer, log probabilities and the way back to the table for 2100 positions, more than the
+    gradient sums unsorted.  Against the same model in 64 bits: 32-bit sums of up to some 2100 terms, each of a dozen operations -
+    the summed roundings stay below 2200 * 2^-24 of the largest value."""
+    units, vocab, ncols, p, seed = 96, 130, 2100, 0.2, 5
+    rng = np.random.default_rng(4)
+    O = cb.dev_dia_matrix_f(vocab, units, np.arange(-60, 60, dtype=np.int32))
+    O.set_vec(rng.standard_normal(O.num_dia * O.stride) * 0.1)
+    table = cb.to_device(rng.standard_normal((units, vocab)))
+    tok, target = (torch.from_numpy(rng.integers(-1, vocab, ncols)).cuda() for _ in range(2))
+    E = cb.colmajor_empty
+    x, y, logits = E(units, ncols), E(units, ncols), E(vocab, ncols)
+    dlogits, dy, dx, dtable = E(vocab, ncols), E(units, ncols), E(units, ncols), torch.ones((vocab, units), device="cuda").t()
+    cb.embedding(x, table, tok, 1.5)
+    cb.dropout(y, x, p, seed, step=1)
+    cb.prod(logits, O, y)
+    r = cb.token_logprob(logits, target, entropy=True)
+    dlogp, dent = torch.full((ncols,), -1.0 / ncols, device="cuda"), torch.full((ncols,), -0.01 / ncols, device="cuda")
+    cb.token_logprob_grad(dlogits, logits, r.lse, target, dlogp, r.entropy, dent)
+    cb.prod(dy, O, dlogits, "t")
+    cb.dropout_grad(dx, dy, p, seed, step=1)
+    cb.embedding_grad(dtable, tok, dx, 1.5)
+    first = dtable.clone()
+    cb.embedding_grad(dtable, tok, dx, 1.5, 1.0)                # a second batch's, added
+
+    keep = torch.from_numpy(ho.uniform(units, ncols, seed, 1) >= np.float32(p)).cuda()
+    t64, O64 = table.double().requires_grad_(), torch.from_numpy(cb.pull(O)).cuda().double()
+    x64 = torch.where(tok >= 0, t64[:, tok.clamp(min=0)] * 1.5, 0.0)
+    logq = torch.log_softmax(O64 @ torch.where(keep, x64 / (1.0 - float(np.float32(p))), 0.0), 0)
+    logp = torch.where(target >= 0, logq.gather(0, target.clamp(min=0)[None])[0], 0.0)
+    (-logp.sum() / ncols + 0.01 / ncols * (logq.exp() * logq).sum()).backward()
+    bound = 2200 * E32 * t64.grad.abs().max()
+    assert (first.double() - t64.grad).abs().max() <= bound
+    assert (dtable.double() - 2 * t64.grad).abs().max() <= 2 * bound
