@@ -1,11 +1,14 @@
 // Log probabilities of given tokens under softmax(scale * logits), column by column, with the log-sum-exp, the entropy
 // and the likeliest tokens; and the gradient with respect to the logits.
 //
-// Everything is held in 32 bits in powers of two: with c = scale * log2(e), the largest logit M of a column and
-// d_v = (logit_v - M) * c (the difference first, so that logits far from zero and masks of the type's lowest value do no harm),
+// Everything is held in 32 bits in powers of two: with c = scale * log2(e), R one of the column's largest logits (below) and
+// d_v = (logit_v - R) * c (the difference first, so that logits far from zero and masks of the type's lowest value do no harm),
 //   s = sum_v 2^d_v        t = sum_v 2^d_v * d_v
-//   lse = scale * M + ln 2 * log2 s      entropy = ln 2 * (log2 s - t / s)      logp_v = scale * (logit_v - M) - ln 2 * log2 s
-// M, s and t come from one pass: a running maximum, and sums that are rescaled by 2^(c * (old M - new M)) when it grows.
+//   lse = scale * R + ln 2 * log2 s      entropy = ln 2 * (log2 s - t / s)      logp_v = scale * (logit_v - R) - ln 2 * log2 s
+// R, s and t come from one pass.  A thread's sums are relative to a logit it has met, and are rescaled by 2^(c * (old R - new R))
+// when that is left behind: at once where alternatives are asked for, so that R is the column's largest logit M; else only when a
+// chunk's sum exceeds 2^24, so that R lies at most 24 powers of two below M.  That bounds what log2 s - t / s and logit_v - R
+// against log2 s lose to cancellation: numbers below 32 have a spacing of 2^-19 at most, some 1e-6 in the results.
 #include <type_traits>
 
 #include "cluster.cuh"
@@ -326,11 +329,15 @@ __device__ __forceinline__ void sum_chunk(const uint4* v, int step, float m0, fl
     }
 }
 
-// Adds a chunk to a thread's sums.  The sums may be relative to any logit that keeps the powers finite, so the maximum is only
-// looked for in a thread's first chunk (MAX: in every chunk, for callers that want the maximum itself).  A chunk whose sums come
-// out beyond 1e30 or NaN - a logit far above the first chunk's, or an exponent of -inf (a forbidden token) times its power of
-// zero - is summed once more, relative to its maximum and with its exponents cut, and so are the thread's later chunks at once
-// (careful); the other threads need no test per element.
+// A chunk's sum beyond this has left its reference behind: 2^24, of exponents of up to 24 times the powers with ENT.  (At 2^16 the
+// logits of a normal distribution with a deviation of 5 exceeded it often enough to cost a tenth of the time, at 2^24 next to never.)
+template <bool ENT> constexpr float OVER = ENT ? 16.f * 16777216.f : 16777216.f;
+
+// Adds a chunk to a thread's sums.  The sums may be relative to any logit not far below the largest, so the maximum is only looked
+// for in a thread's first chunk (MAX: in every chunk, for callers that want the maximum itself).  A chunk whose sum exceeds OVER - a
+// logit far above the reference - or come out NaN - an exponent of -inf (a forbidden token, or the empty end of a column's last
+// chunk) times its power of zero - is summed once more, relative to its maximum and with its exponents cut; after a NaN so are the
+// thread's later chunks at once (careful).  The other threads need no test per element.
 template <class T, bool ENT, bool MAX>
 __device__ __forceinline__ void add_chunk(Sums& a, const uint4* v, int step, float c, Where& w, int at, bool& careful) {
     if (MAX) {
@@ -342,12 +349,15 @@ __device__ __forceinline__ void add_chunk(Sums& a, const uint4* v, int step, flo
         raise<ENT>(a, max_chunk<T>(v, step), c);
     }
     float2 s, t;
+    bool again = careful;
     if (!careful) {
         sum_chunk<T, ENT, false>(v, step, shift(a.m), c, s, t);
-        careful = !(fabsf(ENT ? t.x + t.y : s.x + s.y) < 1e30f);
-        if (careful && !MAX) raise<ENT>(a, max_chunk<T>(v, step), c);
+        const float sum = ENT ? t.x + t.y : s.x + s.y;
+        again = !(sum < OVER<ENT>);
+        careful = sum != sum;
+        if (again && !MAX) raise<ENT>(a, max_chunk<T>(v, step), c);
     }
-    if (careful) sum_chunk<T, ENT, ENT>(v, step, shift(a.m), c, s, t);
+    if (again) sum_chunk<T, ENT, ENT>(v, step, shift(a.m), c, s, t);
     a.s = __fadd2_rn(a.s, s);
     if (ENT) a.t = __fadd2_rn(a.t, t);
 }

@@ -12,7 +12,7 @@ import torch
 
 import cuv_b200 as cb
 from oracle import host_oracle as ho
-from test_gpu_tokens import E32, gen
+from test_gpu_tokens import E32, TYPES, gen, matrix, near, plain_logprob
 
 pytestmark = pytest.mark.gpu
 
@@ -182,3 +182,124 @@ def test_a_token_model_of_many_positions():
     bound = 2200 * E32 * t64.grad.abs().max()
     assert (first.double() - t64.grad).abs().max() <= bound
     assert (dtable.double() - 2 * t64.grad).abs().max() <= 2 * bound
+
+
+# ---- token log probabilities ----------------------------------------------------------------------------------------
+
+FAR = 24 * math.log(2.0)        # how far, at most, the logit that a column's sums are relative to lies below its largest one
+
+
+def check(logits, tokens, scale, top, r):
+    """Against 64 bits.  With z - R the exponents, R at most FAR below the largest z:  a power is off by 2^-22 and by four roundings
+    of its exponent (the difference, log2(e), its product with the scale, the product), once more for what it is rescaled by when
+    the reference grows; sums are taken in at most vocab/128 + 150 additions and rescaled at most vocab/1024 + 40 times, each time
+    by a power and a product.  The logarithm and its product with ln 2 are off by 2^-22 of themselves, which R adds FAR to."""
+    lse, logp, ent, logq, spread = plain_logprob(logits, tokens, scale)
+    vocab, size = logits.shape[0], math.log(logits.shape[0]) + FAR
+    err = (vocab / 1024 + 40) * (2.0 ** -22 + E32) + (vocab / 128 + 150) * E32 + 4 * E32 * (spread + 3 * FAR)
+    near(r.lse, lse, err + 2.0 ** -22 * (lse.abs().nan_to_num(posinf=0.0) + size))
+    if tokens is not None:
+        near(r.logp, logp, err + 2.0 ** -22 * (logp.abs().nan_to_num(posinf=0.0) + size))
+    if r.entropy is not None:
+        near(r.entropy, ent, err * (1 + 2 * (spread + FAR)) + 2.0 ** -22 * (spread + size))
+    if top:
+        ranked = torch.where(torch.isnan(logits.float()), -math.inf, logits.float())
+        value, index = torch.sort(ranked.t(), dim=1, descending=True, stable=True)
+        index = torch.where(value == -math.inf, -1, index)[:, :top]
+        index = torch.nn.functional.pad(index, (0, top - index.shape[1]), value=-1)
+        assert torch.equal(r.top_index, index.int().t())
+        want = torch.where(index < 0, -math.inf, logq.t().gather(1, index.clamp(min=0))).t()
+        near(r.top_logp, want, err + 2.0 ** -22 * (want.abs().nan_to_num(posinf=0.0) + size))
+
+
+# rows and columns: eight lanes, a warp, 128 threads, 256 threads and clusters of 2, 4 and 8 blocks a column
+SHAPES = [(700, 800), (1000, 601), (3000, 2000), (8000, 1300), (40000, 700), (40000, 300), (40000, 40), (131072, 4)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab, ncols", SHAPES)
+@pytest.mark.parametrize("top", [0, 3])
+def test_a_token_far_above_the_others(kind, vocab, ncols, top):
+    """One token anywhere in a column, 40 to 80 above the others, around what a sum of powers can hold too: certain, whatever the
+    sums are relative to.  The others' powers sum up to 2^-25 at most, so each sum that has the token's power of one in it stays one,
+    and what is left is their own share: vocab e^-40 of the log probability, and 80 times that of the entropy."""
+    g, dtype = gen(vocab + top), TYPES[kind]
+    x = (torch.rand((ncols, vocab), device="cuda", generator=g) - 1.0).to(dtype).t()
+    place = torch.randint(0, vocab, (ncols,), device="cuda", generator=g)
+    height = torch.rand(ncols, device="cuda", generator=g) * 40 + 40
+    x.scatter_(0, place[None], height.to(dtype)[None])
+    share = vocab * math.exp(-40.0)
+    assert share < 2.0 ** -25
+    for entropy in (False, True):
+        r = cb.token_logprob(x, place, entropy=entropy, top=top)
+        assert r.logp.abs().max() <= share
+        assert torch.equal(r.lse, x.float().gather(0, place[None])[0])
+        if entropy:
+            assert r.entropy.abs().max() <= 81 * share
+        if top:
+            assert torch.equal(r.top_index[0], place.int()) and torch.equal(r.top_logp[0], r.logp)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab, ncols", SHAPES)
+@pytest.mark.parametrize("top", [0, 1, 20, 32])
+def test_masks_ties_and_specials_on_every_path(kind, vocab, ncols, top):
+    g, dtype, off = gen(vocab * 3 + top), TYPES[kind], vocab % 7 + 1
+
+    def ask(logits, entropy=True):
+        return cb.token_logprob(logits, tok, scale=0.8, entropy=entropy, top=top)
+
+    x, buf = matrix(g, vocab, ncols, dtype, vocab + off, off, spread=6.0)
+    tok = torch.randint(-1, vocab + 1, (ncols,), device="cuda", generator=g)
+    check(x, tok, 0.8, top, ask(x))
+    check(x, tok, 0.8, top, ask(x, False))
+    # the first half far below the rest, not at all, and by more than a sum of powers can hold
+    for low in (-9.0, -30.0, -65.0, -75.0, -200.0):
+        y = x.t().clone().t()
+        y[:vocab // 2] += low
+        check(y, tok, 0.8, top, ask(y))
+        check(y, tok, 0.8, top, ask(y, False))
+    # ties: few different values, then a single one
+    y = torch.randint(0, 3, (ncols, vocab), device="cuda", generator=g).to(dtype).t()
+    check(y, tok, 0.8, top, ask(y))
+    y.fill_(1.5)
+    r = ask(y)
+    check(y, tok, 0.8, top, r)
+    assert r.top_index is None or r.top_index[:, -1].tolist() == list(range(top))
+    # forbidden tokens, the type's lowest value, columns with nothing left
+    x[torch.rand((ncols, vocab), device="cuda", generator=g).t() < 0.5] = -math.inf
+    x[torch.rand(vocab, device="cuda", generator=g) < 0.1] = torch.finfo(dtype).min
+    x[:vocab // 3, ::2] = -math.inf
+    x[:vocab // 3, 1::3] = torch.finfo(dtype).min
+    x[:, 1] = -math.inf
+    x[:, -1] = -math.inf
+    want = ask(x)
+    check(x, tok, 0.8, top, want)
+    check(x, tok, 0.8, top, ask(x, False))
+    assert want.lse[1] == -math.inf and want.entropy[1] == 0
+    # NaN and +inf in single columns, which leave the others as they were
+    x[vocab - 2, 0] = math.nan
+    x[vocab // 2, 2] = math.inf
+    r = ask(x)
+    there = (tok >= 0) & (tok < vocab)
+    for name in ("lse", "logp", "entropy"):
+        a, b = getattr(r, name).clone(), getattr(want, name)
+        for col in (0, 2):
+            assert torch.isnan(a[col]) or name == "logp" and not there[col]
+            a[col] = b[col]
+        assert torch.equal(a, b)
+    if top:
+        rest = [c for c in range(ncols) if c not in (0, 2)]
+        assert r.top_index[0, 2] == vocab // 2 and torch.equal(r.top_index[:, rest], want.top_index[:, rest])
+        assert not (r.top_index[:, 0] == vocab - 2).any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab, ncols", SHAPES)
+def test_far_logits_without_alternatives(kind, vocab, ncols):
+    """Logits around 10000 (1000 in half precision): the differences cancel the offset."""
+    g, dtype = gen(vocab), TYPES[kind]
+    x = (torch.randn((ncols, vocab), device="cuda", generator=g) * 3 + (1000.0 if kind == "f16" else 10000.0)).to(dtype).t()
+    tok = torch.randint(0, vocab, (ncols,), device="cuda", generator=g)
+    for entropy in (False, True):
+        check(x, tok, 1.0, 0, cb.token_logprob(x, tok, entropy=entropy))
