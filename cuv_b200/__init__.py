@@ -665,7 +665,8 @@ def embedding(dst, table, tokens, scale=1.0):
 
 def embedding_grad(dtable, tokens, dout, factNew=1.0, factOld=0.0):
     """dtable[:, v] = factOld*dtable[:, v] + factNew * sum of dout[:, j] over the positions j with tokens[j] == v: the
-    gradient of :func:`embedding` (``factNew`` = its scale) for the whole table, summed in 32 bits in ascending j.
+    gradient of :func:`embedding` (``factNew`` = its scale) for the whole table, summed in 32 bits in a fixed order (ascending j;
+    in a call of more than 256 positions by groups of them, see ``include/cuvdia.h``).
     ``factOld=0`` writes zeros into the columns of tokens that do not occur; ``factOld=1`` leaves those alone.  ``dtable`` has
     the type of ``dout`` or float32."""
     ldo, code, units, ncols, index = _matrix(dout, "dout")

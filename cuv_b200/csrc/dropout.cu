@@ -56,10 +56,11 @@ template <class T> struct Streams { T* dst; const T* src; const T* residual; lon
 // loads are in flight before the first number is drawn.  WIDE: a part is a block's.  NONE: p = 1, every element is dropped.
 //
 // Bound by memory where an element is at least six bytes of traffic: 16384 x 8192 bf16 with residual 117 us (6.9 TB/s), 16384 x 4096
-// f32 80 us (6.7 TB/s).  A 16-bit pass without residual (four bytes) is bound by the generator, whose 17 wide products per four
-// elements fill the multiplier pipe: 107 us at 16384 x 8192 for 82 us of traffic; taking the products' high words from the double
-// units instead gained nothing, the register moves around them costing as much.  Columns that do not start on vectors:
-// 16383 x 8191 with residual 172 us (element by element 315 us).
+// f32 80 us (6.7 TB/s), in short bursts of calls (under a sustained load, at a lower clock, the first takes 128 us).  A 16-bit pass
+// without residual (four bytes) is bound by the generator's 17 wide products per four elements: 103 to 107 us at 16384 x 8192 for
+// 82 us of traffic, its warps waiting for arithmetic and dispatch and hardly for memory; taking the products' high words from the
+// double units instead gained nothing, the register moves around them costing as much.  Columns that do not start on vectors:
+// 16383 x 8191 168 us with residual (element by element 315 us), 154 us without.
 template <class T, bool RESIDUAL, bool SHIFTED, bool NONE, int U, bool WIDE>
 __global__ void __launch_bounds__(256, 4)
 dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts, const DropoutArgs a) {
@@ -173,7 +174,8 @@ dropout_kernel(const Streams<T> m, int rows, int ncols, int log_lanes, int parts
 }
 
 // ---- any layout --------------------------------------------------------------------------------------------------------
-// Matrices that lie differently: four rows, one group of the generator, a thread, element by element.
+// Matrices that lie differently: four rows, one group of the generator, a thread, element by element (16383 x 8191 bf16 221 us with
+// residual, 197 us without; 16383 x 4096 f32 102 us).
 template <class T, bool RESIDUAL>
 __global__ void __launch_bounds__(256)
 dropout_any_kernel(const Streams<T> m, int rows, int ncols, long long groups, bool none, const DropoutArgs a) {

@@ -402,7 +402,8 @@ __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col
 // alone are too few to fill the GPU: its blocks leave their sums and lists in the first block's shared memory, which joins
 // them, so that there is one launch and no scratch memory.
 //
-// Bound by memory where columns are many: 32768 x 8192 bf16 with entropies 82 us (6.5 TB/s; the exponential unit is 80 % busy),
+// Bound by memory where columns are many: 32768 x 8192 bf16 with entropies 82 us (6.5 TB/s; the exponential unit is 80 % busy; in
+// short bursts, under a sustained load at a lower clock 89 us), 32767 x 8192 90 us, whose last chunks have empty places,
 // 50021 x 1000 f32 39 us (5.1 TB/s: 7 blocks on most SMs, 6 on the others, and their common start and end), with 20 alternatives
 // and a third of the tokens forbidden 45 us.  A few columns are bound by latency: 131072 x 4 bf16 6 us, 8.5 us with alternatives.
 template <class T, bool ENT, bool TOP, int TEAM>
@@ -645,7 +646,8 @@ int launch_token_logprob(const void* logits, int ld, int type, int vocab, int nc
 // a column of up to 64.  The stores are vectors too where dlogits lies alike, else element by element.  In place is fine: a
 // thread reads its elements before it writes them.
 // Bound by memory: 32768 x 8192 bf16 with or without entropies 158 us (6.8 TB/s), 32768 x 4096 f32 160 us.  The straight-line path
-// for blocks that lie inside a column is what that took (one path with tests per vector: 176 us).
+// for blocks that lie inside a column is what that took (one path with tests per vector: 176 us).  A result that lies otherwise than
+// the logits on the 16-byte grid is stored element by element: 32768 x 8192 bf16 520 to 600 us, 32768 x 4096 f32 184 us.
 struct GradFactors { float scale, minus_lse, a, b; };
 
 // two gradients but for the token's own term; CUT: exponents are cut, see LEAST

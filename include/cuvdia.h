@@ -429,9 +429,11 @@ CUVDIA_API int cuvdia_sequence_f32(float* dst, long long n, void* stream);
  * the row count are neither read nor written.  Element types: CUVDIA_T_F32, CUVDIA_T_F16,
  * CUVDIA_T_BF16; everything is computed in 32 bits and rounded once.  Tokens: CUVDIA_T_I32 or
  * CUVDIA_T_I64; a token outside [0, vocab) - padding - names no token, which is not an error.  Row
- * counts (units, rows, vocab of the logits) go up to 2^30.  Sums are taken in a fixed order (the same
- * call gives identical bits on every run).  No call allocates; all of them can be recorded into a graph,
- * on their first call too.
+ * counts (units, rows, vocab of the logits) go up to 2^30.  Sums are taken in a fixed order: the same
+ * call gives identical bits on every run.  The order follows from the whole call - the column count picks
+ * how the threads share a column of logits, and all of a batch's tokens how a token's columns are grouped -
+ * so the same column in another batch may come out with other last bits.  No call allocates; all of them
+ * can be recorded into a graph, on their first call too.
  * ------------------------------------------------------------------------------------------- */
 #define CUVDIA_T_F16  4
 #define CUVDIA_T_BF16 5
@@ -443,7 +445,9 @@ CUVDIA_API int cuvdia_embedding(void* dst, int ldd, const void* table, int ldt, 
                                 const void* tokens, int token_type, int ncols, float scale, void* stream);
 
 /* Gradient of the table: dtable[:, v] = factOld * dtable[:, v] + factNew * sum of dout[:, j] over the
- * positions j with tokens[j] == v, in ascending j, for EVERY column v of the table.  factOld == 0:
+ * positions j with tokens[j] == v, for EVERY column v of the table, in 32 bits: one after the other in
+ * ascending j up to 256 positions in the call; beyond, ascending groups of up to 32 of them, whose borders
+ * depend on how often smaller tokens occur, and then the groups' sums in a fixed order.  factOld == 0:
  * dtable is not read, columns of tokens that do not occur become zero.  factOld == 1: only columns of
  * tokens that occur are touched (gradients accumulated over several batches).  grad_type is `type`
  * (dout's) or CUVDIA_T_F32.  The positions are sorted by token inside the call; `workspace` is device
