@@ -56,7 +56,7 @@ template <class T> struct Streams { T* dst; const T* src; const T* residual; lon
 // loads are in flight before the first number is drawn.  WIDE: a part is a block's.  NONE: p = 1, every element is dropped.
 //
 // Bound by memory where an element is at least six bytes of traffic: 16384 x 8192 bf16 with residual 117 us (6.9 TB/s), 16384 x 4096
-// f32 80 us (6.7 TB/s), in short bursts of calls (under a sustained load, at a lower clock, the first takes 128 us).  A 16-bit pass
+// f32 80 us (6.7 TB/s), in short bursts of calls (under a sustained load, at a lower clock, the first takes 128 to 136 us).  A 16-bit pass
 // without residual (four bytes) is bound by the generator's 17 wide products per four elements: 103 to 107 us at 16384 x 8192 for
 // 82 us of traffic, its warps waiting for arithmetic and dispatch and hardly for memory; taking the products' high words from the
 // double units instead gained nothing, the register moves around them costing as much.  Columns that do not start on vectors:

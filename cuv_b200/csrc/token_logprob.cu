@@ -403,7 +403,7 @@ __device__ __forceinline__ void write_column(const LogprobArgs& q, long long col
 // them, so that there is one launch and no scratch memory.
 //
 // Bound by memory where columns are many: 32768 x 8192 bf16 with entropies 82 us (6.5 TB/s; the exponential unit is 80 % busy; in
-// short bursts, under a sustained load at a lower clock 89 us), 32767 x 8192 90 us, whose last chunks have empty places,
+// short bursts, under a sustained load at a lower clock 89 to 96 us), 32767 x 8192 90 us, whose last chunks have empty places,
 // 50021 x 1000 f32 39 us (5.1 TB/s: 7 blocks on most SMs, 6 on the others, and their common start and end), with 20 alternatives
 // and a third of the tokens forbidden 45 us.  A few columns are bound by latency: 131072 x 4 bf16 6 us, 8.5 us with alternatives.
 template <class T, bool ENT, bool TOP, int TEAM>
