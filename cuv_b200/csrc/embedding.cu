@@ -388,9 +388,9 @@ sort_move_kernel(const Tokens tokens, const int* __restrict__ keys, const int* _
 // write the columns of tokens that do not occur, 32 columns each: stores that fill the memory's time between the loads.
 // Bound by memory but for the joins and what the sums' launch does not hide of the sort: 4096 x 32768 f32 from 16384 bf16 columns
 // 129 us (103 us of traffic), 1024 x 131072 from 8192 bf16 57 us (44 us).  Columns off 16-byte boundaries go element by element:
-// 4095 x 32768 149 us.  factOld = 1 saves the absent columns and reads the others: 96 us (47 us of traffic), but 1023 x 50021 from
-// 8191 f32 132 us (with factOld = 0: 59 us), whose single elements are read one after the other.  Longer chunks leave fewer partial sums but too few warps: with blocks
-// that sum 64 columns each the first took 237 us.
+// 4095 x 32768 149 us.  factOld = 1 saves the absent columns and reads the others, in the middle of the sums: 96 us (47 us of
+// traffic), but 1023 x 50021 from 8191 f32 132 us (with factOld = 0 59 us).  Longer chunks leave fewer partial sums but too few
+// warps: with blocks that sum 64 columns each the first took 237 us.
 
 constexpr int LONG_JOIN = 8;            // more partial sums than this are shared out among a block's warps
 
